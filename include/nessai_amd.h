@@ -631,6 +631,57 @@ NSA_API int nsa_train_backward(const long long* plan, const int* tables_dev, con
                                const float* g_logdet_dev, const float* g_log_prob_dev, float* gx_out_dev,
                                void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Operators around a conditional flow: what a net that makes its context is built from and trained with (the reference
+ * leaves these to torch: the flow takes any `context` tensor, src/nessai/flows/base.py:236-245, and its training loop
+ * calls torch.nn.utils.clip_grad_norm_, src/nessai/flowmodel/base.py:437-441).
+ * Every call enqueues its work on `stream` and returns; device pointers must belong to the current device.
+ * ------------------------------------------------------------------------------------------------------------- */
+enum { NSA_DT_F32 = 0, NSA_DT_BF16 = 1, NSA_DT_F16 = 2 };                       /* types of values */
+enum { NSA_NORM_L1 = 1, NSA_NORM_L2 = 2, NSA_NORM_INF = 3 };                    /* kinds of norms */
+enum { NSA_FN_NONE = -1, NSA_FN_RELU = 0, NSA_FN_TANH = 1, NSA_FN_SILU = 2 };   /* activations */
+
+/* norm_out_dev[0] = the norm over all elements of `count` tensors (tensors[i]: device pointer, sizes[i] contiguous
+ * elements of type dtypes[i]; the three arrays are host memory and are read before the call returns).  A tensor listed
+ * twice counts twice.  nsa_grad_clip then multiplies every element by min(1, max_norm / (norm + 1e-6)); there two
+ * tensors must not overlap (NSA_E_ARG).  workspace_dev: nsa_grad_norm_workspace(count) bytes, 8-byte aligned. */
+NSA_API size_t nsa_grad_norm_workspace(int count);
+NSA_API int nsa_grad_norm(int count, void* const* tensors, const long long* sizes, const int* dtypes, int kind,
+                          void* workspace_dev, size_t workspace_bytes, float* norm_out_dev, void* stream);
+NSA_API int nsa_grad_clip(int count, void* const* tensors, const long long* sizes, const int* dtypes, int kind,
+                          float max_norm, void* workspace_dev, size_t workspace_bytes, float* norm_out_dev, void* stream);
+
+/* Group norm with an activation, channels last: x [samples][length][channels], groups of channels / groups neighbouring
+ * channels, mean and (biased) variance over a sample's positions and a group's channels,
+ *   y = act(((x - mean) / sqrt(var + eps)) * weight[c] + bias[c]).
+ * weight_dev / bias_dev: [channels] of type weight_dtype (float32 or x's type), or NULL.  mean_dev / rstd_dev:
+ * [samples][groups] float32, written by the forward call and read by the backward call.  The backward call writes the
+ * gradients whose pointers dx_dev, dweight_dev, dbias_dev are not NULL (the parameters' in type weight_dtype).
+ * workspace_dev: nsa_group_norm_workspace(...) bytes, 16-byte aligned. */
+NSA_API size_t nsa_group_norm_workspace(long long samples, long long length, int channels, int groups, int dtype,
+                                        int backward);
+NSA_API int nsa_group_norm_forward(long long samples, long long length, int channels, int groups, int dtype,
+                                   const void* x_dev, int weight_dtype, const void* weight_dev, const void* bias_dev,
+                                   float eps, int activation, void* y_dev, float* mean_dev, float* rstd_dev,
+                                   void* workspace_dev, size_t workspace_bytes, void* stream);
+NSA_API int nsa_group_norm_backward(long long samples, long long length, int channels, int groups, int dtype,
+                                    const void* x_dev, const void* dy_dev, int weight_dtype, const void* weight_dev,
+                                    const void* bias_dev, int activation, const float* mean_dev, const float* rstd_dev,
+                                    void* dx_dev, void* dweight_dev, void* dbias_dev, void* workspace_dev,
+                                    size_t workspace_bytes, void* stream);
+
+/* Embedding: out[i] = weight[ids[i]] * scale, rows of `width` values; ids are int32 (ids_bytes 4) or int64 (8).  An id
+ * outside [0, vocab) gives a row of NaN and takes no part in the gradient.
+ * Gradient: dweight[v] = scale * sum over i with ids[i] == v of dy[i] (float32 sums in the order of i, rounded once);
+ * every row is written, those without a token and row `padding` (none: -1) with zeros.
+ * workspace_dev: nsa_embedding_workspace(...) bytes, 16-byte aligned. */
+NSA_API int nsa_embedding_forward(long long tokens, long long vocab, int width, int dtype, const void* ids_dev,
+                                  int ids_bytes, const void* weight_dev, float scale, void* out_dev, void* stream);
+NSA_API size_t nsa_embedding_workspace(long long tokens, long long vocab, int width, int dtype);
+NSA_API int nsa_embedding_backward(long long tokens, long long vocab, int width, int dtype, const void* ids_dev,
+                                   int ids_bytes, const void* dy_dev, float scale, long long padding, void* dweight_dev,
+                                   void* workspace_dev, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

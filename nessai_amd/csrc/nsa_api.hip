@@ -35,7 +35,7 @@
 
 static thread_local char g_err[512] = "";
 
-static int nsa_fail(int code, const char* fmt, ...) {
+int nsa_fail(int code, const char* fmt, ...) {  // (nsa_elem.h declares it for the other files of the library)
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(g_err, sizeof(g_err), fmt, ap);

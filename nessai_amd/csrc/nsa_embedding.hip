@@ -1,0 +1,440 @@
+// Embedding lookup with scaling, and its gradient by sorted tokens.
+//
+//   out[i] = W[id_i] * scale                      dW[v] = scale * sum_{i : id_i = v} dy[i]
+//
+// The lookup moves rows: a team of lanes takes a row, 16 bytes to a lane where rows and addresses allow it.
+//
+// The gradient must add the rows of equal ids.  Float atomics would add them in an order that changes from run to run, so
+// the tokens are sorted by id first - a stable radix sort of (id, position), 8 bits to a pass, as many passes as the
+// table's size has digits - and the sums then run over neighbours, in the order of the positions: equal inputs give equal
+// bits.  The sorted list is cut into chunks of equal length, whatever the frequencies of the ids: an id inside one chunk
+// is finished there; one that runs over a chunk's border leaves float32 partial sums, which a second kernel joins.
+#include <hip/hip_runtime.h>
+#include <algorithm>
+
+#include "nsa_elem.h"
+
+#define EMB_THREADS 256
+#define EMB_ITEMS 16                          // keys per thread of a sorting tile
+#define EMB_TILE (EMB_THREADS * EMB_ITEMS)
+#define EMB_CHUNK 32                          // sorted positions per team of the reduction
+
+// ---------------------------------------------------------------------------
+// lookup
+// ---------------------------------------------------------------------------
+
+template <typename T, typename ID, int V>
+__global__ void __launch_bounds__(EMB_THREADS) emb_lookup(long long tokens, long long vocab, int width,
+                                                          const ID* __restrict__ ids, const T* __restrict__ weight,
+                                                          float scale, int lanes, T* __restrict__ out) {
+  const int teams = EMB_THREADS / lanes, lane = threadIdx.x % lanes;
+  for (long long row = (long long)blockIdx.x * teams + threadIdx.x / lanes; row < tokens; row += (long long)gridDim.x * teams) {
+    const long long id = (long long)ids[row];
+    const bool known = id >= 0 && id < vocab;
+    for (int c = lane * V; c < width; c += lanes * V) {
+      float v[V];
+      if (known) {
+        nsa_load<T, V>(weight + id * width + c, v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] *= scale;
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = __builtin_nanf("");
+      }
+      nsa_store<T, V>(out + row * width + c, v);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// stable radix sort of (id, position)
+// ---------------------------------------------------------------------------
+
+// the key of a token: its id, or `vocab` (behind every row) for a token without a gradient
+template <typename ID>
+__device__ __forceinline__ uint32_t emb_key(const ID* ids, long long i, long long vocab, long long padding) {
+  const long long id = (long long)ids[i];
+  return id >= 0 && id < vocab && id != padding ? (uint32_t)id : (uint32_t)vocab;
+}
+
+// digit counts of every tile: counts[digit][tile]; the first pass reads the ids themselves (keys == nullptr)
+template <typename ID>
+__global__ void __launch_bounds__(EMB_THREADS) emb_count(int n, const ID* __restrict__ ids, long long vocab,
+                                                         long long padding, const uint32_t* __restrict__ keys, int shift,
+                                                         uint32_t* __restrict__ counts) {
+  __shared__ uint32_t bins[256];
+  bins[threadIdx.x] = 0;
+  __syncthreads();
+  const long long base = (long long)blockIdx.x * EMB_TILE;
+  for (int k = 0; k < EMB_ITEMS; ++k) {
+    const long long i = base + k * EMB_THREADS + threadIdx.x;
+    if (i < n) {
+      const uint32_t key = keys != nullptr ? keys[i] : emb_key(ids, i, vocab, padding);
+      atomicAdd(&bins[(key >> shift) & 255u], 1u);
+    }
+  }
+  __syncthreads();
+  counts[(long long)threadIdx.x * gridDim.x + blockIdx.x] = bins[threadIdx.x];
+}
+
+// one workgroup per digit: its tiles' counts become the counts in front of them, totals[digit] their sum
+__global__ void __launch_bounds__(EMB_THREADS) emb_scan(int tiles, uint32_t* __restrict__ counts,
+                                                        uint32_t* __restrict__ totals) {
+  __shared__ uint32_t wave_sum[EMB_THREADS / 64];
+  uint32_t* row = counts + (long long)blockIdx.x * tiles;
+  uint32_t carry = 0;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int base = 0; base < tiles; base += EMB_THREADS) {
+    const int i = base + threadIdx.x;
+    const uint32_t v = i < tiles ? row[i] : 0u;
+    uint32_t s = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t t = __shfl_up(s, o);
+      if (lane >= o) s += t;
+    }
+    if (lane == 63) wave_sum[wave] = s;
+    __syncthreads();
+    uint32_t before = carry, all = 0;
+    for (int w = 0; w < EMB_THREADS / 64; ++w) {
+      if (w < wave) before += wave_sum[w];
+      all += wave_sum[w];
+    }
+    if (i < tiles) row[i] = before + s - v;
+    carry += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) totals[blockIdx.x] = carry;
+}
+
+// The tile's keys to their places.  Each wave owns a contiguous quarter of the tile and counts its digits first; the place
+// of a key is then (keys of smaller digits) + (the digit's keys in earlier tiles, in earlier waves, in earlier rounds of
+// this wave, in lower lanes): equal digits keep their order.
+template <typename ID>
+__global__ void __launch_bounds__(EMB_THREADS) emb_scatter(int n, const ID* __restrict__ ids, long long vocab,
+                                                           long long padding, const uint32_t* __restrict__ keys,
+                                                           const uint32_t* __restrict__ pos, int shift,
+                                                           const uint32_t* __restrict__ counts,
+                                                           const uint32_t* __restrict__ totals,
+                                                           uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out) {
+  constexpr int WAVES = EMB_THREADS / 64;
+  __shared__ uint32_t place[WAVES][256];
+  __shared__ uint32_t wave_sum[WAVES];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int w = 0; w < WAVES; ++w) place[w][threadIdx.x] = 0;
+  // keys of smaller digits: an exclusive scan of the 256 totals, one digit per thread
+  const uint32_t total = totals[threadIdx.x];
+  uint32_t s = total;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t t = __shfl_up(s, o);
+    if (lane >= o) s += t;
+  }
+  if (lane == 63) wave_sum[wave] = s;
+  __syncthreads();
+  uint32_t first = s - total;
+  for (int w = 0; w < wave; ++w) first += wave_sum[w];
+
+  const long long base = (long long)blockIdx.x * EMB_TILE + wave * (64 * EMB_ITEMS) + lane;
+  uint32_t key[EMB_ITEMS], from[EMB_ITEMS];
+#pragma unroll
+  for (int k = 0; k < EMB_ITEMS; ++k) {
+    const long long i = base + k * 64;
+    key[k] = from[k] = 0;
+    if (i < n) {
+      key[k] = keys != nullptr ? keys[i] : emb_key(ids, i, vocab, padding);
+      from[k] = pos != nullptr ? pos[i] : (uint32_t)i;
+      atomicAdd(&place[wave][(key[k] >> shift) & 255u], 1u);
+    }
+  }
+  __syncthreads();
+  uint32_t at = first + counts[(long long)threadIdx.x * gridDim.x + blockIdx.x];
+  for (int w = 0; w < WAVES; ++w) {
+    const uint32_t c = place[w][threadIdx.x];
+    place[w][threadIdx.x] = at;
+    at += c;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < EMB_ITEMS; ++k) {
+    const bool here = base + k * 64 < n;
+    const uint32_t digit = (key[k] >> shift) & 255u;
+    unsigned long long same = __ballot(here);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      const unsigned long long set = __ballot((digit >> b) & 1u);
+      same &= (digit >> b) & 1u ? set : ~set;
+    }
+    const uint32_t rank = __popcll(same & ((1ULL << lane) - 1ULL));
+    if (here) {
+      const uint32_t to = __hip_atomic_load(&place[wave][digit], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) + rank;
+      keys_out[to] = key[k];
+      pos_out[to] = from[k];
+    }
+    __builtin_amdgcn_wave_barrier();  // every lane has read its place before the round's count is added
+    if (here && rank == 0) atomicAdd(&place[wave][digit], (uint32_t)__popcll(same));
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// sums over equal ids
+// ---------------------------------------------------------------------------
+
+template <typename T>
+__global__ void __launch_bounds__(EMB_THREADS) emb_zero(long long n, T* __restrict__ p) {
+  for (long long i = (long long)blockIdx.x * EMB_THREADS + threadIdx.x; i < n; i += (long long)gridDim.x * EMB_THREADS)
+    p[i] = (T)0.0f;
+}
+
+// A team of `lanes` lanes takes EMB_CHUNK sorted positions, V columns to a lane.  slots[chunk][0]: the partial sum of an id
+// that began in an earlier chunk; [1]: of one that began here and goes on in the next.
+template <typename T, int V>
+__global__ void __launch_bounds__(EMB_THREADS) emb_reduce(int n, uint32_t vocab, int width, int lanes,
+                                                          const uint32_t* __restrict__ keys,
+                                                          const uint32_t* __restrict__ pos, const T* __restrict__ dy,
+                                                          float scale, T* __restrict__ dweight,
+                                                          float* __restrict__ slots) {
+  const int teams = EMB_THREADS / lanes;
+  const long long chunk = (long long)blockIdx.x * teams + threadIdx.x / lanes;
+  const long long begin = chunk * EMB_CHUNK;
+  if (begin >= n) return;
+  const long long end = begin + EMB_CHUNK < n ? begin + EMB_CHUNK : n;
+  const bool goes_on = end < n && keys[end] == keys[end - 1];
+  for (int c = (blockIdx.y * lanes + threadIdx.x % lanes) * V; c < width; c += gridDim.y * lanes * V) {
+    float acc[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] = 0.0f;
+    uint32_t key = keys[begin];
+    bool earlier = begin > 0 && keys[begin - 1] == key;
+    for (long long i = begin; i < end; ++i) {
+      float row[V];
+      if (key != vocab) {
+        nsa_load<T, V>(dy + (long long)pos[i] * width + c, row);
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] += row[v];
+      }
+      const uint32_t next = i + 1 < end ? keys[i + 1] : 0u;
+      if (i + 1 < end && next == key) continue;
+      if (key != vocab) {
+        const bool later = i + 1 == end && goes_on;
+        if (earlier || later) {
+          nsa_store<float, V>(slots + (2 * chunk + (earlier ? 0 : 1)) * width + c, acc);
+        } else {
+#pragma unroll
+          for (int v = 0; v < V; ++v) acc[v] *= scale;
+          nsa_store<T, V>(dweight + (long long)key * width + c, acc);
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = 0.0f;
+      key = next;
+      earlier = false;
+    }
+  }
+}
+
+// One workgroup per chunk border: the id that goes over it is summed by the chunk in which it begins.
+template <typename T>
+__global__ void __launch_bounds__(EMB_THREADS) emb_join(int n, uint32_t vocab, int width, const uint32_t* __restrict__ keys,
+                                                        float scale, const float* __restrict__ slots,
+                                                        T* __restrict__ dweight) {
+  const long long chunk = blockIdx.x, begin = chunk * EMB_CHUNK, end = begin + EMB_CHUNK;  // end < n: a border
+  const uint32_t key = keys[end - 1];
+  if (key == vocab || keys[end] != key) return;
+  if (begin > 0 && keys[begin - 1] == key && keys[begin] == key) return;  // it began earlier
+  // the end of its run, by bisection
+  long long lo = end, hi = n;
+  while (hi - lo > 1) {
+    const long long m = (lo + hi) >> 1;
+    if (keys[m] == key) lo = m;
+    else hi = m;
+  }
+  const long long last = lo / EMB_CHUNK;
+  for (int c = threadIdx.x; c < width; c += EMB_THREADS) {
+    float acc = slots[(2 * chunk + 1) * width + c];
+    for (long long k = chunk + 1; k <= last; ++k) acc += slots[2 * k * width + c];
+    dweight[(long long)key * width + c] = (T)(acc * scale);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+namespace {
+
+// the widest access, in elements, that rows of `width` elements at these addresses allow
+int emb_vector(int width, int bytes, uintptr_t addresses) {
+  int v = 16 / bytes;
+  while (v > 1 && (width % v != 0 || addresses % (uintptr_t)(v * bytes) != 0)) v >>= 1;
+  return v;
+}
+
+// lanes of a team: a power of two up to a wave that leaves few lanes idle in a row of `vectors` accesses
+int emb_lanes(int vectors) {
+  int best = 1;
+  for (int l = 1; l <= 64; l <<= 1) {
+    const int rounds = (vectors + l - 1) / l;
+    if (rounds * l * 8 <= vectors * 9 || l <= vectors / 2) best = l;  // at most an eighth idle, or two rounds and more
+  }
+  return vectors == 1 ? 1 : best;
+}
+
+int emb_passes(long long vocab) {  // 8 bits each; the largest key is `vocab` itself
+  int bits = 1;
+  while (bits < 32 && (vocab >> bits) != 0) ++bits;
+  return (bits + 7) / 8;
+}
+
+struct EmbSpace {
+  uint32_t *keys[2], *pos[2], *counts, *totals;
+  float* slots;
+  size_t bytes;
+};
+
+EmbSpace emb_space(char* p, long long n, int width) {
+  EmbSpace w;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    char* q = p + at;
+    at += (bytes + 255) & ~(size_t)255;
+    return q;
+  };
+  const long long tiles = (n + EMB_TILE - 1) / EMB_TILE, chunks = (n + EMB_CHUNK - 1) / EMB_CHUNK;
+  for (int i = 0; i < 2; ++i) {
+    w.keys[i] = (uint32_t*)take(n * 4);
+    w.pos[i] = (uint32_t*)take(n * 4);
+  }
+  w.counts = (uint32_t*)take(tiles * 256 * 4);
+  w.totals = (uint32_t*)take(256 * 4);
+  w.slots = (float*)take((size_t)chunks * 2 * width * 4);
+  w.bytes = at;
+  return w;
+}
+
+int emb_check(const char* what, long long tokens, long long vocab, int width, int dtype, int ids_bytes) {
+  if (tokens < 0 || vocab < 1 || width < 1) return nsa_fail(NSA_E_ARG, "%s: bad size", what);
+  if (tokens >= (1LL << 31) || vocab >= (1LL << 31))
+    return nsa_fail(NSA_E_ARG, "%s: at most 2^31 - 1 tokens and rows", what);
+  if (!nsa_elem_known(dtype)) return nsa_fail(NSA_E_ARG, "%s: unknown type %d", what, dtype);
+  if (ids_bytes != 4 && ids_bytes != 8) return nsa_fail(NSA_E_ARG, "%s: ids are int32 or int64", what);
+  return NSA_OK;
+}
+
+int emb_done(const char* what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? NSA_OK : nsa_fail(NSA_E_HIP, "%s: %s", what, hipGetErrorString(e));
+}
+
+template <typename T, typename ID, int V>
+void emb_lookup_launch(long long tokens, long long vocab, int width, const void* ids, const void* weight, float scale,
+                       void* out, hipStream_t s) {
+  const int lanes = emb_lanes((width + V - 1) / V), teams = EMB_THREADS / lanes;
+  const long long groups = (tokens + teams - 1) / teams;
+  hipLaunchKernelGGL((emb_lookup<T, ID, V>), dim3((unsigned)std::min(groups, 65536LL)), dim3(EMB_THREADS), 0, s, tokens,
+                     vocab, width, (const ID*)ids, (const T*)weight, scale, lanes, (T*)out);
+}
+
+template <typename T, typename ID>
+void emb_lookup_typed(long long tokens, long long vocab, int width, const void* ids, const void* weight, float scale,
+                      void* out, hipStream_t s) {
+  const int v = emb_vector(width, sizeof(T), (uintptr_t)weight | (uintptr_t)out);
+  if constexpr (sizeof(T) == 2) {
+    if (v == 8) return emb_lookup_launch<T, ID, 8>(tokens, vocab, width, ids, weight, scale, out, s);
+  }
+  if (v == 4) return emb_lookup_launch<T, ID, 4>(tokens, vocab, width, ids, weight, scale, out, s);
+  if (v == 2) return emb_lookup_launch<T, ID, 2>(tokens, vocab, width, ids, weight, scale, out, s);
+  emb_lookup_launch<T, ID, 1>(tokens, vocab, width, ids, weight, scale, out, s);
+}
+
+template <typename T, int V>
+void emb_reduce_launch(int n, long long vocab, int width, const EmbSpace& w, int side, const void* dy, float scale,
+                       void* dweight, hipStream_t s) {
+  const int lanes = emb_lanes((width + V - 1) / V), teams = EMB_THREADS / lanes;
+  const long long chunks = ((long long)n + EMB_CHUNK - 1) / EMB_CHUNK;
+  const int slabs = std::min((width + lanes * V - 1) / (lanes * V), 64);
+  hipLaunchKernelGGL((emb_reduce<T, V>), dim3((unsigned)((chunks + teams - 1) / teams), slabs), dim3(EMB_THREADS), 0, s, n,
+                     (uint32_t)vocab, width, lanes, w.keys[side], w.pos[side], (const T*)dy, scale, (T*)dweight, w.slots);
+  const long long borders = ((long long)n - 1) / EMB_CHUNK;
+  if (borders > 0)
+    hipLaunchKernelGGL((emb_join<T>), dim3((unsigned)borders), dim3(EMB_THREADS), 0, s, n, (uint32_t)vocab, width,
+                       w.keys[side], scale, w.slots, (T*)dweight);
+}
+
+template <typename ID>
+int emb_sort(int n, long long vocab, const ID* ids, long long padding, const EmbSpace& w, hipStream_t s) {
+  const unsigned tiles = (unsigned)(((long long)n + EMB_TILE - 1) / EMB_TILE);
+  const int passes = emb_passes(vocab);
+  for (int p = 0; p < passes; ++p) {
+    const uint32_t* keys = p == 0 ? nullptr : w.keys[p & 1];
+    const uint32_t* pos = p == 0 ? nullptr : w.pos[p & 1];
+    hipLaunchKernelGGL((emb_count<ID>), dim3(tiles), dim3(EMB_THREADS), 0, s, n, ids, vocab, padding, keys, 8 * p, w.counts);
+    hipLaunchKernelGGL(emb_scan, dim3(256), dim3(EMB_THREADS), 0, s, (int)tiles, w.counts, w.totals);
+    hipLaunchKernelGGL((emb_scatter<ID>), dim3(tiles), dim3(EMB_THREADS), 0, s, n, ids, vocab, padding, keys, pos, 8 * p,
+                       w.counts, w.totals, w.keys[(p + 1) & 1], w.pos[(p + 1) & 1]);
+  }
+  return passes & 1;
+}
+
+template <typename T>
+void emb_backward_typed(int n, long long vocab, int width, const void* ids, int ids_bytes, const void* dy, float scale,
+                        long long padding, void* dweight, const EmbSpace& w, hipStream_t s) {
+  const long long cells = vocab * width;
+  hipLaunchKernelGGL((emb_zero<T>), dim3((unsigned)std::min((cells + EMB_THREADS - 1) / EMB_THREADS, 8192LL)),
+                     dim3(EMB_THREADS), 0, s, cells, (T*)dweight);
+  if (n == 0) return;
+  const int side = ids_bytes == 4 ? emb_sort<int>(n, vocab, (const int*)ids, padding, w, s)
+                                  : emb_sort<long long>(n, vocab, (const long long*)ids, padding, w, s);
+  const int v = emb_vector(width, sizeof(T), (uintptr_t)dy | (uintptr_t)dweight);
+  if constexpr (sizeof(T) == 2) {
+    if (v == 8) return emb_reduce_launch<T, 8>(n, vocab, width, w, side, dy, scale, dweight, s);
+  }
+  if (v == 4) return emb_reduce_launch<T, 4>(n, vocab, width, w, side, dy, scale, dweight, s);
+  if (v == 2) return emb_reduce_launch<T, 2>(n, vocab, width, w, side, dy, scale, dweight, s);
+  emb_reduce_launch<T, 1>(n, vocab, width, w, side, dy, scale, dweight, s);
+}
+
+}  // namespace
+
+extern "C" NSA_API int nsa_embedding_forward(long long tokens, long long vocab, int width, int dtype, const void* ids_dev,
+                                             int ids_bytes, const void* weight_dev, float scale, void* out_dev,
+                                             void* stream) {
+  if (const int rc = emb_check("nsa_embedding_forward", tokens, vocab, width, dtype, ids_bytes)) return rc;
+  if (tokens == 0) return NSA_OK;
+  if (!ids_dev || !weight_dev || !out_dev) return nsa_fail(NSA_E_ARG, "nsa_embedding_forward: NULL argument");
+  hipStream_t s = (hipStream_t)stream;
+#define EMB_LOOKUP(T)                                                                                              \
+  (ids_bytes == 4 ? emb_lookup_typed<T, int>(tokens, vocab, width, ids_dev, weight_dev, scale, out_dev, s)           \
+                  : emb_lookup_typed<T, long long>(tokens, vocab, width, ids_dev, weight_dev, scale, out_dev, s))
+  if (dtype == NSA_DT_F32) EMB_LOOKUP(float);
+  else if (dtype == NSA_DT_BF16) EMB_LOOKUP(nsa_bf16);
+  else EMB_LOOKUP(nsa_f16);
+#undef EMB_LOOKUP
+  return emb_done("nsa_embedding_forward");
+}
+
+extern "C" NSA_API size_t nsa_embedding_workspace(long long tokens, long long vocab, int width, int dtype) {
+  (void)vocab;
+  (void)dtype;
+  if (tokens <= 0 || width <= 0) return 0;
+  return emb_space(nullptr, tokens, width).bytes;
+}
+
+extern "C" NSA_API int nsa_embedding_backward(long long tokens, long long vocab, int width, int dtype, const void* ids_dev,
+                                              int ids_bytes, const void* dy_dev, float scale, long long padding,
+                                              void* dweight_dev, void* workspace_dev, size_t workspace_bytes,
+                                              void* stream) {
+  if (const int rc = emb_check("nsa_embedding_backward", tokens, vocab, width, dtype, ids_bytes)) return rc;
+  if (!dweight_dev) return nsa_fail(NSA_E_ARG, "nsa_embedding_backward: NULL argument");
+  if (tokens > 0 && (!ids_dev || !dy_dev || !workspace_dev))
+    return nsa_fail(NSA_E_ARG, "nsa_embedding_backward: NULL argument");
+  if (workspace_bytes < nsa_embedding_workspace(tokens, vocab, width, dtype))
+    return nsa_fail(NSA_E_ARG, "nsa_embedding_backward: workspace too small");
+  const EmbSpace w = emb_space((char*)workspace_dev, tokens, width);
+  hipStream_t s = (hipStream_t)stream;
+  const int n = (int)tokens;
+  if (dtype == NSA_DT_F32) emb_backward_typed<float>(n, vocab, width, ids_dev, ids_bytes, dy_dev, scale, padding, dweight_dev, w, s);
+  else if (dtype == NSA_DT_BF16) emb_backward_typed<nsa_bf16>(n, vocab, width, ids_dev, ids_bytes, dy_dev, scale, padding, dweight_dev, w, s);
+  else emb_backward_typed<nsa_f16>(n, vocab, width, ids_dev, ids_bytes, dy_dev, scale, padding, dweight_dev, w, s);
+  return emb_done("nsa_embedding_backward");
+}

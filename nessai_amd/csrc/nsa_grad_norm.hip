@@ -1,0 +1,279 @@
+// The norm over many gradient tensors and the clip that follows it:
+//   T = (sum |g|^p)^(1/p), p = 1, 2 or infinity, over every element of every tensor
+//   g <- g * min(1, max_norm / (T + 1e-6))      (rounded once to the gradient's type)
+// as torch.nn.utils.clip_grad_norm_ does in the reference's loop (src/nessai/flowmodel/base.py:437-441).
+//
+// Both are bound by memory: the norm reads every gradient once, the clip reads and writes it once more because the
+// factor is known only after the last element.  What many small tensors cost is launches, so the tensors are merged
+// into runs (neighbours in memory become one), the runs travel as kernel arguments, NG_RUNS of them per launch, and
+// every workgroup takes an equal, contiguous share of the launch's elements whatever the tensors' sizes are.  The
+// shares are read in a fixed order and their partial sums added in a fixed order: equal inputs at equal places give equal
+// bits.  Squares and sums are held in 64 bits: a square of a float32 over- or underflows in 32.
+#include <hip/hip_runtime.h>
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "nsa_elem.h"
+
+#define NG_RUNS 160          // runs per launch: 2 x 8 bytes each, inside the 4 KB of a kernel's arguments
+#define NG_THREADS 256
+#define NG_BLOCKS 2048       // workgroups of a launch at most: 8 per compute unit ...
+#define NG_BLOCKS_MIN 128    // ... and fewer where there are many launches: every partial sum is read by all of them
+#define NG_SHARE 4096        // elements of a workgroup's share: a multiple of this
+
+struct NgRuns {
+  long long first[NG_RUNS + 1];  // elements in front of run k
+  void* ptr[NG_RUNS];
+  int count;
+};
+
+// |a| and |b| -> the larger one, NaN if either is one (fmaxf drops it)
+__device__ __forceinline__ float ng_max(float a, float b) { return (a > b || a != a) ? a : b; }
+
+template <int KIND>
+struct NgAcc {
+  double s = 0.0;
+  __device__ __forceinline__ void add(float v) {
+    if constexpr (KIND == NSA_NORM_L2) s = fma((double)v, (double)v, s);
+    else if constexpr (KIND == NSA_NORM_L1) s += (double)fabsf(v);
+    else s = (double)ng_max((float)s, fabsf(v));
+  }
+  __device__ __forceinline__ void join(double o) {
+    if constexpr (KIND == NSA_NORM_INF) s = (s > o || s != s) ? s : o;
+    else s += o;
+  }
+};
+
+template <int KIND, int THREADS>
+__device__ __forceinline__ double ng_block_join(double s) {  // the sum on every thread, in a fixed order
+  __shared__ double part[THREADS / 64];
+  NgAcc<KIND> a;
+  a.s = s;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) a.join(__shfl_xor(a.s, o));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = a.s;
+  __syncthreads();
+  NgAcc<KIND> all;
+  all.s = part[0];
+#pragma unroll
+  for (int w = 1; w < THREADS / 64; ++w) all.join(part[w]);
+  __syncthreads();
+  return all.s;
+}
+
+// the elements [lo, hi) of the launch, run by run: f(pointer, length), each a contiguous piece
+template <typename F>
+__device__ __forceinline__ void ng_pieces(const NgRuns& r, long long lo, long long hi, F f) {
+  int a = 0, b = r.count;  // first[a] <= lo < first[b]
+  while (b - a > 1) {
+    const int m = (a + b) >> 1;
+    if (r.first[m] <= lo) a = m;
+    else b = m;
+  }
+  while (lo < hi) {
+    const long long end = r.first[a + 1] < hi ? r.first[a + 1] : hi;
+    f(r.ptr[a], lo - r.first[a], end - lo);
+    lo = end;
+    ++a;
+  }
+}
+
+template <typename T, int KIND>
+__global__ void __launch_bounds__(NG_THREADS) ng_partial(NgRuns r, long long share, double* __restrict__ partial) {
+  NgAcc<KIND> acc;
+  const long long lo = blockIdx.x * share;
+  const long long hi = lo + share < r.first[r.count] ? lo + share : r.first[r.count];
+  ng_pieces(r, lo, hi, [&](const void* base, long long at, long long len) {
+    const T* p = (const T*)base + at;
+    for (long long i = threadIdx.x; i < len; i += NG_THREADS) acc.add((float)p[i]);
+  });
+  const double s = ng_block_join<KIND, NG_THREADS>(acc.s);
+  if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+template <int KIND>
+__device__ __forceinline__ float ng_total(const double* __restrict__ partial, int n_partial) {
+  NgAcc<KIND> acc;
+  for (int i = threadIdx.x; i < n_partial; i += NG_THREADS) acc.join(partial[i]);
+  const double s = ng_block_join<KIND, NG_THREADS>(acc.s);
+  return (float)(KIND == NSA_NORM_L2 ? sqrt(s) : s);
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(NG_THREADS) ng_finish(const double* __restrict__ partial, int n_partial,
+                                                        float* __restrict__ norm_out) {
+  const float norm = ng_total<KIND>(partial, n_partial);
+  if (threadIdx.x == 0) norm_out[0] = norm;
+}
+
+// min(1, max_norm / (norm + 1e-6)) in float32, NaN kept
+__device__ __forceinline__ float ng_factor(float norm, float max_norm) {
+  const float f = max_norm / (norm + 1e-6f);
+  return f > 1.0f ? 1.0f : f;
+}
+
+// Every workgroup adds up the partial sums by itself (at most a few thousand values out of the L2 cache, in the same
+// order everywhere) instead of waiting for one that does: one launch less between the norm and the product.
+template <typename T, int KIND>
+__global__ void __launch_bounds__(NG_THREADS) ng_scale(NgRuns r, long long share, const double* __restrict__ partial,
+                                                       int n_partial, float max_norm, float* __restrict__ norm_out) {
+  const float norm = ng_total<KIND>(partial, n_partial);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && norm_out != nullptr) norm_out[0] = norm;
+  const float f = ng_factor(norm, max_norm);
+  if (f == 1.0f) return;  // (a product by one changes nothing)
+  const long long lo = blockIdx.x * share;
+  const long long hi = lo + share < r.first[r.count] ? lo + share : r.first[r.count];
+  ng_pieces(r, lo, hi, [&](void* base, long long at, long long len) {
+    T* p = (T*)base + at;
+    for (long long i = threadIdx.x; i < len; i += NG_THREADS) p[i] = (T)((float)p[i] * f);
+  });
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+namespace {
+
+struct Run {
+  char* ptr;
+  long long n;
+  int dtype;
+};
+
+// The tensors as runs, in the order of their places, tensors side by side merged.  false: two of them overlap.
+bool ng_runs(int count, void* const* tensors, const long long* sizes, const int* dtypes, std::vector<Run>& runs) {
+  runs.clear();
+  runs.reserve(count);
+  for (int i = 0; i < count; ++i)
+    if (sizes[i] > 0) runs.push_back({(char*)tensors[i], sizes[i], dtypes[i]});
+  std::sort(runs.begin(), runs.end(), [](const Run& a, const Run& b) { return a.ptr < b.ptr; });
+  bool apart = true;
+  size_t kept = 0;
+  for (size_t i = 0; i < runs.size(); ++i) {
+    if (kept > 0) {
+      Run& last = runs[kept - 1];
+      char* end = last.ptr + last.n * nsa_elem_bytes(last.dtype);
+      if (runs[i].ptr < end) apart = false;
+      if (runs[i].ptr == end && runs[i].dtype == last.dtype) {
+        last.n += runs[i].n;
+        continue;
+      }
+    }
+    runs[kept++] = runs[i];
+  }
+  runs.resize(kept);
+  std::stable_sort(runs.begin(), runs.end(), [](const Run& a, const Run& b) { return a.dtype < b.dtype; });
+  return apart;
+}
+
+struct Launch {
+  NgRuns r;
+  int dtype, blocks;
+  long long share;
+};
+
+void ng_launches(const std::vector<Run>& runs, std::vector<Launch>& out) {
+  out.clear();
+  for (size_t i = 0; i < runs.size();) {
+    Launch l;
+    l.dtype = runs[i].dtype;
+    l.r.count = 0;
+    l.r.first[0] = 0;
+    while (i < runs.size() && l.r.count < NG_RUNS && runs[i].dtype == l.dtype) {
+      l.r.ptr[l.r.count] = runs[i].ptr;
+      l.r.first[l.r.count + 1] = l.r.first[l.r.count] + runs[i].n;
+      ++l.r.count;
+      ++i;
+    }
+    out.push_back(l);
+  }
+  const int blocks = std::max(NG_BLOCKS_MIN, 2 * NG_BLOCKS / (int)(out.size() + 1));
+  for (Launch& l : out) {
+    const long long total = l.r.first[l.r.count], shares = (total + NG_SHARE - 1) / NG_SHARE;
+    l.share = (shares + blocks - 1) / blocks * NG_SHARE;
+    l.blocks = (int)((total + l.share - 1) / l.share);
+  }
+}
+
+#define NG_KINDS(T, KERNEL, ...)                                                    \
+  switch (kind) {                                                                   \
+    case NSA_NORM_L1: hipLaunchKernelGGL((KERNEL<T, NSA_NORM_L1>), __VA_ARGS__); break;   \
+    case NSA_NORM_L2: hipLaunchKernelGGL((KERNEL<T, NSA_NORM_L2>), __VA_ARGS__); break;   \
+    default: hipLaunchKernelGGL((KERNEL<T, NSA_NORM_INF>), __VA_ARGS__); break;           \
+  }
+#define NG_DISPATCH(dtype, KERNEL, ...)                              \
+  switch (dtype) {                                                   \
+    case NSA_DT_F32: NG_KINDS(float, KERNEL, __VA_ARGS__) break;     \
+    case NSA_DT_BF16: NG_KINDS(nsa_bf16, KERNEL, __VA_ARGS__) break; \
+    default: NG_KINDS(nsa_f16, KERNEL, __VA_ARGS__) break;           \
+  }
+
+int ng_run(const char* what, int count, void* const* tensors, const long long* sizes, const int* dtypes, int kind,
+           bool clip, float max_norm, double* workspace, size_t workspace_bytes, float* norm_out, hipStream_t s) {
+  if (count < 0 || (count > 0 && (!tensors || !sizes || !dtypes)) || !norm_out || !workspace)
+    return nsa_fail(NSA_E_ARG, "%s: NULL argument", what);
+  if (kind != NSA_NORM_L1 && kind != NSA_NORM_L2 && kind != NSA_NORM_INF)
+    return nsa_fail(NSA_E_ARG, "%s: unknown norm %d", what, kind);
+  if (clip && !(max_norm >= 0.0f)) return nsa_fail(NSA_E_ARG, "%s: max_norm must not be negative or NaN", what);
+  for (int i = 0; i < count; ++i) {
+    if (!nsa_elem_known(dtypes[i])) return nsa_fail(NSA_E_ARG, "%s: unknown type %d of tensor %d", what, dtypes[i], i);
+    if (sizes[i] < 0 || (sizes[i] > 0 && !tensors[i])) return nsa_fail(NSA_E_ARG, "%s: bad tensor %d", what, i);
+    if ((uintptr_t)tensors[i] % nsa_elem_bytes(dtypes[i]) != 0)
+      return nsa_fail(NSA_E_ARG, "%s: tensor %d is not aligned to its elements", what, i);
+  }
+  if (workspace_bytes < nsa_grad_norm_workspace(count))
+    return nsa_fail(NSA_E_ARG, "%s: workspace too small", what);
+  try {
+    std::vector<Run> runs;
+    std::vector<Launch> launches;
+    const bool apart = ng_runs(count, tensors, sizes, dtypes, runs);
+    if (clip && !apart) return nsa_fail(NSA_E_ARG, "%s: two gradients overlap in memory", what);
+    ng_launches(runs, launches);
+    int n_partial = 0;
+    for (const Launch& l : launches) {
+      NG_DISPATCH(l.dtype, ng_partial, dim3(l.blocks), dim3(NG_THREADS), 0, s, l.r, l.share, workspace + n_partial)
+      n_partial += l.blocks;
+    }
+    if (!clip || launches.empty()) {
+      if (kind == NSA_NORM_L1)
+        hipLaunchKernelGGL(ng_finish<NSA_NORM_L1>, dim3(1), dim3(NG_THREADS), 0, s, workspace, n_partial, norm_out);
+      else if (kind == NSA_NORM_L2)
+        hipLaunchKernelGGL(ng_finish<NSA_NORM_L2>, dim3(1), dim3(NG_THREADS), 0, s, workspace, n_partial, norm_out);
+      else
+        hipLaunchKernelGGL(ng_finish<NSA_NORM_INF>, dim3(1), dim3(NG_THREADS), 0, s, workspace, n_partial, norm_out);
+    } else {
+      float* out = norm_out;
+      for (const Launch& l : launches) {
+        NG_DISPATCH(l.dtype, ng_scale, dim3(l.blocks), dim3(NG_THREADS), 0, s, l.r, l.share, workspace, n_partial,
+                    max_norm, out)
+        out = nullptr;
+      }
+    }
+  } catch (const std::bad_alloc&) {
+    return nsa_fail(NSA_E_ARG, "%s: out of host memory", what);
+  }
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? NSA_OK : nsa_fail(NSA_E_HIP, "%s: %s", what, hipGetErrorString(e));
+}
+
+}  // namespace
+
+extern "C" NSA_API size_t nsa_grad_norm_workspace(int count) {
+  // one partial sum per workgroup of every launch; the three types make at most two launches more
+  const size_t launches = (size_t)(count > 0 ? count : 0) / NG_RUNS + 3;
+  return launches * NG_BLOCKS * sizeof(double);
+}
+
+extern "C" NSA_API int nsa_grad_norm(int count, void* const* tensors, const long long* sizes, const int* dtypes, int kind,
+                                     void* workspace_dev, size_t workspace_bytes, float* norm_out_dev, void* stream) {
+  return ng_run("nsa_grad_norm", count, tensors, sizes, dtypes, kind, false, 0.0f, (double*)workspace_dev, workspace_bytes,
+                norm_out_dev, (hipStream_t)stream);
+}
+
+extern "C" NSA_API int nsa_grad_clip(int count, void* const* tensors, const long long* sizes, const int* dtypes, int kind,
+                                     float max_norm, void* workspace_dev, size_t workspace_bytes, float* norm_out_dev,
+                                     void* stream) {
+  return ng_run("nsa_grad_clip", count, tensors, sizes, dtypes, kind, true, max_norm, (double*)workspace_dev,
+                workspace_bytes, norm_out_dev, (hipStream_t)stream);
+}

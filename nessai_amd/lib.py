@@ -176,6 +176,32 @@ SIGNATURES = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
          c_void_p, c_void_p],
     ),
+    "nsa_grad_norm_workspace": (c_size_t, [c_int]),
+    "nsa_grad_norm": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "nsa_grad_clip": (
+        c_int,
+        [c_int, c_void_p, c_void_p, c_void_p, c_int, c_float, c_void_p, c_size_t, c_void_p, c_void_p],
+    ),
+    "nsa_group_norm_workspace": (c_size_t, [c_ll, c_ll, c_int, c_int, c_int, c_int]),
+    "nsa_group_norm_forward": (
+        c_int,
+        [c_ll, c_ll, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_float, c_int, c_void_p, c_void_p,
+         c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
+    "nsa_group_norm_backward": (
+        c_int,
+        [c_ll, c_ll, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+         c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
+    "nsa_embedding_forward": (
+        c_int,
+        [c_ll, c_ll, c_int, c_int, c_void_p, c_int, c_void_p, c_float, c_void_p, c_void_p],
+    ),
+    "nsa_embedding_workspace": (c_size_t, [c_ll, c_ll, c_int, c_int]),
+    "nsa_embedding_backward": (
+        c_int,
+        [c_ll, c_ll, c_int, c_int, c_void_p, c_int, c_void_p, c_float, c_ll, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
     "nsa_populate_accept": (
         c_int,
         [c_ll, c_int, c_void_p, c_void_p, c_ull, c_ull, c_void_p, c_void_p, c_ll, c_void_p, c_void_p,

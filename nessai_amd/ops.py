@@ -17,6 +17,10 @@ the two differentiable ones into autograd:
                                  gradients (``nsa_train_backward``)
 ===============================  =========================================================
 
+Beside the flow stand the operators that a net which makes a flow's context is built from and
+trained with (``nessai_amd.ops_context``): ``embedding``, ``group_norm_act``, ``grad_norm`` and
+``clip_grad_norm_``.
+
 There is no CPU implementation: the operators exist for the ``CUDA`` (ROCm) dispatch key
 only, plus ``Meta`` shape functions.
 """
@@ -260,3 +264,8 @@ def header_tensor(header):
     """Host int32 tensor holding the 32-bit header words bit for bit (operator argument of ``flow_run``, which
     hands its address to the library: no per-call conversion)."""
     return torch.from_numpy(np.frombuffer(bytes(header), dtype=np.uint32).view(np.int32).copy())
+
+
+# -- operators of a context net (nessai_amd.ops_context) ------------------------------------
+
+from .ops_context import clip_grad_norm_, embedding, grad_norm, group_norm_act  # noqa: E402,F401

@@ -1,0 +1,117 @@
+"""Refusals of the operators around the flow (``nessai_amd.ops``: ``embedding``, ``group_norm_act``, ``grad_norm``,
+``clip_grad_norm_``) and of their C entry points.  All of them are decided on the host: no device is needed."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from nessai_amd import lib, ops
+
+
+def test_group_norm_act_refuses_what_it_cannot_compute():
+    x = torch.randn(4, 5, 12)
+    with pytest.raises(ValueError, match="cannot be divided"):
+        ops.group_norm_act(x, 5)
+    with pytest.raises(ValueError, match="cannot be divided"):
+        ops.group_norm_act(x, 0)
+    with pytest.raises(ValueError, match="shape"):
+        ops.group_norm_act(torch.randn(12), 3)
+    with pytest.raises(ValueError, match="Unknown activation"):
+        ops.group_norm_act(x, 3, activation="gelu")
+    with pytest.raises(ValueError, match="weight"):
+        ops.group_norm_act(x, 3, weight=torch.ones(11))
+    with pytest.raises(ValueError, match="bias"):
+        ops.group_norm_act(x, 3, bias=torch.ones(1, 12))
+    with pytest.raises(ValueError, match="eps"):
+        ops.group_norm_act(x, 3, eps=-1.0)
+    with pytest.raises(ValueError, match="eps"):
+        ops.group_norm_act(x, 3, eps=math.nan)
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        ops.group_norm_act(x.double(), 3)
+    with pytest.raises(TypeError, match="x's type"):
+        ops.group_norm_act(x, 3, weight=torch.ones(12, dtype=torch.bfloat16))
+    with pytest.raises(TypeError, match="one type"):
+        ops.group_norm_act(x.bfloat16(), 3, torch.ones(12), torch.ones(12, dtype=torch.bfloat16))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.group_norm_act(x, 3)
+
+
+def test_embedding_refuses_what_it_cannot_compute():
+    w, i = torch.randn(7, 3), torch.tensor([1, 2])
+    with pytest.raises(TypeError, match="int32 or int64"):
+        ops.embedding(i.float(), w)
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        ops.embedding(i, w.double())
+    with pytest.raises(ValueError, match="table of shape"):
+        ops.embedding(i, w[0])
+    with pytest.raises(ValueError, match="table of shape"):
+        ops.embedding(i, w[:0])
+    for bad in (7, -8):
+        with pytest.raises(ValueError, match="padding_idx"):
+            ops.embedding(i, w, padding_idx=bad)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.embedding(i, w)
+
+
+def test_gradient_norm_refuses_what_it_cannot_compute():
+    p = torch.nn.Parameter(torch.randn(3))
+    assert float(ops.clip_grad_norm_([p], 1.0)) == 0.0 and float(ops.grad_norm([])) == 0.0  # nothing to clip
+    p.grad = torch.randn(3)
+    with pytest.raises(ValueError, match="norm_type"):
+        ops.clip_grad_norm_([p], 1.0, norm_type=3)
+    with pytest.raises(ValueError, match="norm_type"):
+        ops.grad_norm([p.grad], norm_type=0.5)
+    for bad in (-1.0, math.nan):
+        with pytest.raises(ValueError, match="max_norm"):
+            ops.clip_grad_norm_([p], bad)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.clip_grad_norm_(p, 1.0)
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        ops.grad_norm(torch.randn(3, dtype=torch.float64))
+    with pytest.raises(TypeError, match="dense"):
+        ops.grad_norm(torch.eye(3).to_sparse())
+
+
+def _norm_args(places, sizes, codes):
+    n = len(places)
+    return (n, (ctypes.c_void_p * n)(*places), (ctypes.c_longlong * n)(*sizes), (ctypes.c_int * n)(*codes))
+
+
+def test_entry_points_check_their_arguments_before_anything_is_launched():
+    L = lib.load()
+    ws, out = 4096, 8192  # addresses that no call below reaches
+    size = L.nsa_grad_norm_workspace(2)
+    assert L.nsa_grad_norm_workspace(10_000) >= size > 0
+    for places, sizes, codes, kind, max_norm, bytes_, message in (
+        ((16, 32), (4, 5), (0, 7), 2, 1.0, size, b"unknown type"),
+        ((16, 32), (4, -1), (0, 0), 2, 1.0, size, b"bad tensor"),
+        ((16, None), (4, 1), (0, 0), 2, 1.0, size, b"bad tensor"),
+        ((16, 34), (4, 5), (0, 0), 2, 1.0, size, b"aligned"),
+        ((16, 32), (4, 5), (0, 0), 9, 1.0, size, b"unknown norm"),
+        ((16, 32), (4, 5), (0, 0), 2, -1.0, size, b"max_norm"),
+        ((16, 32), (4, 5), (0, 0), 2, math.nan, size, b"max_norm"),
+        ((16, 32), (4, 5), (0, 0), 2, 1.0, size - 1, b"workspace"),
+        ((16, 28), (4, 5), (0, 0), 2, 1.0, size, b"overlap"),
+        ((16, 16), (4, 4), (0, 0), 2, 1.0, size, b"overlap"),
+        ((16, 24), (2, 20), (0, 1), 2, 1.0, 0, b"workspace"),
+        ((64, 16), (4, 100), (0, 1), 2, 1.0, size, b"overlap"),
+    ):
+        args = _norm_args(places, sizes, codes)
+        assert L.nsa_grad_clip(*args, kind, max_norm, ws, bytes_, out, None) < 0
+        assert message in L.nsa_last_error(), (message, L.nsa_last_error())
+    assert L.nsa_group_norm_forward(2, 3, 12, 5, 0, ws, 0, None, None, 1e-5, -1, ws, ws, ws, ws, 1 << 20, None) < 0
+    assert b"multiple of groups" in L.nsa_last_error()
+    assert L.nsa_group_norm_forward(2, 3, 12, 4, 0, ws, 1, None, None, 1e-5, -1, ws, ws, ws, ws, 1 << 20, None) < 0
+    assert L.nsa_group_norm_forward(2, 3, 12, 4, 0, ws, 0, None, None, 1e-5, 7, ws, ws, ws, ws, 1 << 20, None) < 0
+    assert L.nsa_group_norm_forward(2, 3, 12, 4, 0, None, 0, None, None, 1e-5, -1, ws, ws, ws, ws, 1 << 20, None) < 0
+    assert L.nsa_group_norm_forward(2, 3, 12, 4, 0, ws, 0, None, None, 1e-5, -1, ws, ws, ws, ws, 0, None) < 0
+    assert b"workspace" in L.nsa_last_error()
+    assert L.nsa_group_norm_backward(2, 3, 12, 4, 0, ws, ws, 0, None, None, -1, ws, ws, ws, None, None, ws, 0, None) < 0
+    assert L.nsa_group_norm_workspace(2, 3, 12, 5, 0, 0) == 0
+    assert L.nsa_embedding_forward(4, 0, 8, 0, ws, 8, ws, 1.0, ws, None) < 0
+    assert L.nsa_embedding_forward(1 << 31, 4, 8, 0, ws, 8, ws, 1.0, ws, None) < 0
+    assert L.nsa_embedding_forward(4, 4, 8, 0, ws, 2, ws, 1.0, ws, None) < 0
+    assert L.nsa_embedding_backward(4, 4, 8, 0, ws, 8, ws, 1.0, -1, ws, ws, 0, None) < 0
+    assert b"workspace" in L.nsa_last_error()
+    assert L.nsa_embedding_backward(4, 4, 8, 0, ws, 8, None, 1.0, -1, ws, ws, 1 << 20, None) < 0
