@@ -17,7 +17,8 @@
 #define EMB_THREADS 256
 #define EMB_ITEMS 16                          // keys per thread of a sorting tile
 #define EMB_TILE (EMB_THREADS * EMB_ITEMS)
-#define EMB_CHUNK 32                          // sorted positions per team of the reduction
+#define EMB_AHEAD 8                           // rows in flight per team
+#define EMB_FEW 64                            // rows of a table whose gradient is summed in LDS (64 KB)
 
 // ---------------------------------------------------------------------------
 // lookup
@@ -187,62 +188,77 @@ __global__ void __launch_bounds__(EMB_THREADS) emb_zero(long long n, T* __restri
     p[i] = (T)0.0f;
 }
 
-// A team of `lanes` lanes takes EMB_CHUNK sorted positions, V columns to a lane.  slots[chunk][0]: the partial sum of an id
-// that began in an earlier chunk; [1]: of one that began here and goes on in the next.
+// A team of `lanes` lanes takes a chunk of sorted positions, V columns to a lane; EMB_AHEAD rows are asked for before the first
+// is added.  slots[chunk][0]: the partial sum of an id that began in an earlier chunk; [1]: of one that began here and
+// goes on in the next.
 template <typename T, int V>
-__global__ void __launch_bounds__(EMB_THREADS) emb_reduce(int n, uint32_t vocab, int width, int lanes,
+__global__ void __launch_bounds__(EMB_THREADS) emb_reduce(int n, uint32_t vocab, int width, int lanes, int chunk_len,
                                                           const uint32_t* __restrict__ keys,
                                                           const uint32_t* __restrict__ pos, const T* __restrict__ dy,
                                                           float scale, T* __restrict__ dweight,
                                                           float* __restrict__ slots) {
   const int teams = EMB_THREADS / lanes;
   const long long chunk = (long long)blockIdx.x * teams + threadIdx.x / lanes;
-  const long long begin = chunk * EMB_CHUNK;
-  if (begin >= n) return;
-  const long long end = begin + EMB_CHUNK < n ? begin + EMB_CHUNK : n;
-  const bool goes_on = end < n && keys[end] == keys[end - 1];
-  for (int c = (blockIdx.y * lanes + threadIdx.x % lanes) * V; c < width; c += gridDim.y * lanes * V) {
-    float acc[V];
+  const long long begin = chunk * chunk_len;
+  const int c = (blockIdx.y * lanes + threadIdx.x % lanes) * V;
+  if (begin >= n || c >= width) return;
+  const int len = begin + chunk_len < n ? chunk_len : (int)(n - begin);
+  const bool goes_on = begin + len < n && keys[begin + len] == keys[begin + len - 1];
+  float acc[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] = 0.0f;
-    uint32_t key = keys[begin];
-    bool earlier = begin > 0 && keys[begin - 1] == key;
-    for (long long i = begin; i < end; ++i) {
-      float row[V];
-      if (key != vocab) {
-        nsa_load<T, V>(dy + (long long)pos[i] * width + c, row);
+  for (int v = 0; v < V; ++v) acc[v] = 0.0f;
+  uint32_t key = keys[begin];
+  bool earlier = begin > 0 && keys[begin - 1] == key;
+  auto leave = [&](bool later) {  // the sum of `key` to where it belongs
+    if (key != vocab) {
+      if (earlier || later) {
+        nsa_store<float, V>(slots + (2 * chunk + (earlier ? 0 : 1)) * width + c, acc);
+      } else {
+        float out[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] += row[v];
+        for (int v = 0; v < V; ++v) out[v] = acc[v] * scale;
+        nsa_store<T, V>(dweight + (long long)key * width + c, out);
       }
-      const uint32_t next = i + 1 < end ? keys[i + 1] : 0u;
-      if (i + 1 < end && next == key) continue;
-      if (key != vocab) {
-        const bool later = i + 1 == end && goes_on;
-        if (earlier || later) {
-          nsa_store<float, V>(slots + (2 * chunk + (earlier ? 0 : 1)) * width + c, acc);
-        } else {
+    }
+  };
+  for (int i = 0; i < len; i += EMB_AHEAD) {
+    uint32_t k[EMB_AHEAD];
+    NsaPack<T, V> row[EMB_AHEAD];
 #pragma unroll
-          for (int v = 0; v < V; ++v) acc[v] *= scale;
-          nsa_store<T, V>(dweight + (long long)key * width + c, acc);
-        }
+    for (int j = 0; j < EMB_AHEAD; ++j) {
+      const long long at = begin + (i + j < len ? i + j : len - 1);
+      k[j] = keys[at];
+      row[j] = *reinterpret_cast<const NsaPack<T, V>*>(dy + (long long)pos[at] * width + c);
+    }
+#pragma unroll
+    for (int j = 0; j < EMB_AHEAD; ++j) {
+      if (i + j >= len) break;
+      if (k[j] != key) {
+        leave(false);
+        key = k[j];
+        earlier = false;
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] = 0.0f;
       }
 #pragma unroll
-      for (int v = 0; v < V; ++v) acc[v] = 0.0f;
-      key = next;
-      earlier = false;
+      for (int v = 0; v < V; ++v) acc[v] += (float)row[j].v[v];
     }
   }
+  leave(goes_on);
 }
 
-// One workgroup per chunk border: the id that goes over it is summed by the chunk in which it begins.
+// One workgroup per chunk border: the id that goes over it is summed by the chunk in which it begins.  Long runs are shared by
+// the workgroup's parts, each a row of `lanes` threads; their sums are added in order.
+#define EMB_JOIN_THREADS 512
 template <typename T>
-__global__ void __launch_bounds__(EMB_THREADS) emb_join(int n, uint32_t vocab, int width, const uint32_t* __restrict__ keys,
-                                                        float scale, const float* __restrict__ slots,
-                                                        T* __restrict__ dweight) {
-  const long long chunk = blockIdx.x, begin = chunk * EMB_CHUNK, end = begin + EMB_CHUNK;  // end < n: a border
+__global__ void __launch_bounds__(EMB_JOIN_THREADS) emb_join(int n, uint32_t vocab, int width, int lanes, int chunk_len,
+                                                             const uint32_t* __restrict__ keys, float scale,
+                                                             const float* __restrict__ slots, T* __restrict__ dweight) {
+  __shared__ float sums[EMB_JOIN_THREADS];
+  const long long chunk = blockIdx.x, begin = chunk * chunk_len, end = begin + chunk_len;  // end < n: a border
   const uint32_t key = keys[end - 1];
   if (key == vocab || keys[end] != key) return;
-  if (begin > 0 && keys[begin - 1] == key && keys[begin] == key) return;  // it began earlier
+  if (begin > 0 && keys[begin - 1] == key) return;  // it began earlier
   // the end of its run, by bisection
   long long lo = end, hi = n;
   while (hi - lo > 1) {
@@ -250,12 +266,99 @@ __global__ void __launch_bounds__(EMB_THREADS) emb_join(int n, uint32_t vocab, i
     if (keys[m] == key) lo = m;
     else hi = m;
   }
-  const long long last = lo / EMB_CHUNK;
-  for (int c = threadIdx.x; c < width; c += EMB_THREADS) {
-    float acc = slots[(2 * chunk + 1) * width + c];
-    for (long long k = chunk + 1; k <= last; ++k) acc += slots[2 * k * width + c];
-    dweight[(long long)key * width + c] = (T)(acc * scale);
+  const long long last = lo / chunk_len;
+  const int parts = EMB_JOIN_THREADS / lanes, part = threadIdx.x / lanes;
+  for (int base = 0; base < width; base += lanes) {
+    const int c = base + threadIdx.x % lanes;
+    float acc = 0.0f;
+    if (c < width) {
+#pragma unroll 8
+      for (long long k = chunk + 1 + part; k <= last; k += parts) acc += slots[2 * k * width + c];
+    }
+    sums[threadIdx.x] = acc;
+    __syncthreads();
+    if (part == 0 && c < width) {
+      acc += slots[(2 * chunk + 1) * width + c];
+      for (int p = 1; p < parts; ++p) acc += sums[p * lanes + threadIdx.x];
+      dweight[(long long)key * width + c] = (T)(acc * scale);
+    }
+    __syncthreads();
   }
+}
+
+// ---------------------------------------------------------------------------
+// tables of a few rows: no sorting
+// ---------------------------------------------------------------------------
+
+// A table of up to EMB_FEW rows fits in LDS many times over: every lane keeps a copy of its own columns for all rows and adds
+// its tokens there, in their order - no two lanes ever add to the same place.  A row takes `lanes` lanes, W columns (4
+// bytes) each; a wave works on 64 / lanes tokens at a time.  The copies of a workgroup are added in order and left as
+// part[block][row][column].
+template <typename T, typename ID, int W>
+__global__ void __launch_bounds__(EMB_THREADS) emb_few(long long tokens, int vocab, int width, int lanes, long long share,
+                                                       const ID* __restrict__ ids, long long padding,
+                                                       const T* __restrict__ dy, float* __restrict__ part) {
+  extern __shared__ float acc[];  // [vocab][EMB_THREADS][W]
+  const int cells = vocab * EMB_THREADS * W;
+  for (int i = threadIdx.x; i < cells; i += EMB_THREADS) acc[i] = 0.0f;
+  __syncthreads();
+  const int c = (blockIdx.y * lanes + threadIdx.x % lanes) * W;
+  const int teams = EMB_THREADS / lanes, team = threadIdx.x / lanes;
+  const long long lo = blockIdx.x * share, hi = lo + share < tokens ? lo + share : tokens;
+  float* mine = acc + threadIdx.x * W;
+  if (c < width) {
+    for (long long i = lo + team; i < hi; i += (long long)teams * EMB_AHEAD) {
+      long long id[EMB_AHEAD];
+      NsaPack<T, W> row[EMB_AHEAD];
+#pragma unroll
+      for (int j = 0; j < EMB_AHEAD; ++j) {
+        const long long at = i + (long long)j * teams < hi ? i + (long long)j * teams : i;
+        id[j] = (long long)ids[at];
+        row[j] = *reinterpret_cast<const NsaPack<T, W>*>(dy + at * width + c);
+      }
+#pragma unroll
+      for (int j = 0; j < EMB_AHEAD; ++j) {
+        if (i + (long long)j * teams < hi && id[j] >= 0 && id[j] < vocab && id[j] != padding) {
+          float* p = mine + (int)id[j] * EMB_THREADS * W;
+#pragma unroll
+          for (int w = 0; w < W; ++w) p[w] += (float)row[j].v[w];
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int span = lanes * W;
+  for (int i = threadIdx.x; i < vocab * span; i += EMB_THREADS) {
+    const int row = i / span, e = i - row * span, col = blockIdx.y * span + e;
+    if (col >= width) continue;
+    float s = 0.0f;
+    for (int t = 0; t < teams; ++t) s += acc[(row * EMB_THREADS + t * lanes) * W + e];
+    part[((long long)blockIdx.x * vocab + row) * width + col] = s;
+  }
+}
+
+// dweight = scale * sum over the workgroups' records, in 64 bits
+#define EMB_SUM_THREADS 1024
+#define EMB_SUM_CELLS 32
+template <typename T>
+__global__ void __launch_bounds__(EMB_SUM_THREADS) emb_few_join(int cells, int count, const float* __restrict__ part,
+                                                                float scale, T* __restrict__ dweight) {
+  constexpr int LANES = EMB_SUM_THREADS / EMB_SUM_CELLS;
+  __shared__ double red[EMB_SUM_THREADS];
+  const int i = blockIdx.x * EMB_SUM_CELLS + threadIdx.x % EMB_SUM_CELLS, lane = threadIdx.x / EMB_SUM_CELLS;
+  double s = 0.0;
+  if (i < cells) {
+#pragma unroll 4
+    for (int k = lane; k < count; k += LANES) s += (double)part[(long long)k * cells + i];
+  }
+  red[threadIdx.x] = s;
+  __syncthreads();
+#pragma unroll
+  for (int half = LANES / 2; half > 0; half >>= 1) {
+    if (lane < half) red[threadIdx.x] += red[threadIdx.x + half * EMB_SUM_CELLS];
+    __syncthreads();
+  }
+  if (lane == 0 && i < cells) dweight[i] = (T)(float)(red[threadIdx.x] * (double)scale);
 }
 
 // ---------------------------------------------------------------------------
@@ -286,6 +389,37 @@ int emb_passes(long long vocab) {  // 8 bits each; the largest key is `vocab` it
   return (bits + 7) / 8;
 }
 
+// sorted positions per team of the reduction: short chunks for few tokens (all compute units at work), longer ones for many
+// (fewer partial sums to join)
+int emb_chunk(long long n) {
+  int len = 16;
+  while (len < 256 && n / len > 16384) len *= 2;
+  return len;
+}
+
+// the few-rows form: lanes per row (4-byte accesses; a power of two), and the tokens of a workgroup
+struct EmbFew {
+  bool use;
+  int words, lanes, slabs, blocks;  // words: columns per lane
+  long long share;
+};
+
+EmbFew emb_few_plan(long long n, long long vocab, int width, int bytes) {
+  EmbFew f;
+  f.words = bytes == 2 && width % 2 == 0 ? 2 : 1;
+  f.use = vocab * f.words <= EMB_FEW && n > 0;
+  if (!f.use) return f;
+  const int vectors = width / f.words;
+  f.lanes = 1;
+  while (f.lanes < 64 && f.lanes < vectors) f.lanes *= 2;
+  f.slabs = (vectors + f.lanes - 1) / f.lanes;
+  const long long step = (long long)(EMB_THREADS / f.lanes) * EMB_AHEAD;  // tokens of a workgroup in flight
+  const long long blocks = std::max(1LL, std::min(1024LL / f.slabs + 1, n / (4 * step)));
+  f.share = (n + blocks - 1) / blocks;
+  f.blocks = (int)((n + f.share - 1) / f.share);
+  return f;
+}
+
 struct EmbSpace {
   uint32_t *keys[2], *pos[2], *counts, *totals;
   float* slots;
@@ -300,7 +434,7 @@ EmbSpace emb_space(char* p, long long n, int width) {
     at += (bytes + 255) & ~(size_t)255;
     return q;
   };
-  const long long tiles = (n + EMB_TILE - 1) / EMB_TILE, chunks = (n + EMB_CHUNK - 1) / EMB_CHUNK;
+  const long long tiles = (n + EMB_TILE - 1) / EMB_TILE, chunks = (n + emb_chunk(n) - 1) / emb_chunk(n);
   for (int i = 0; i < 2; ++i) {
     w.keys[i] = (uint32_t*)take(n * 4);
     w.pos[i] = (uint32_t*)take(n * 4);
@@ -350,15 +484,29 @@ void emb_lookup_typed(long long tokens, long long vocab, int width, const void* 
 template <typename T, int V>
 void emb_reduce_launch(int n, long long vocab, int width, const EmbSpace& w, int side, const void* dy, float scale,
                        void* dweight, hipStream_t s) {
-  const int lanes = emb_lanes((width + V - 1) / V), teams = EMB_THREADS / lanes;
-  const long long chunks = ((long long)n + EMB_CHUNK - 1) / EMB_CHUNK;
-  const int slabs = std::min((width + lanes * V - 1) / (lanes * V), 64);
+  const int lanes = emb_lanes((width + V - 1) / V), teams = EMB_THREADS / lanes, len = emb_chunk(n);
+  const long long chunks = ((long long)n + len - 1) / len;
+  const int slabs = (width + lanes * V - 1) / (lanes * V);
   hipLaunchKernelGGL((emb_reduce<T, V>), dim3((unsigned)((chunks + teams - 1) / teams), slabs), dim3(EMB_THREADS), 0, s, n,
-                     (uint32_t)vocab, width, lanes, w.keys[side], w.pos[side], (const T*)dy, scale, (T*)dweight, w.slots);
-  const long long borders = ((long long)n - 1) / EMB_CHUNK;
+                     (uint32_t)vocab, width, lanes, len, w.keys[side], w.pos[side], (const T*)dy, scale, (T*)dweight,
+                     w.slots);
+  const long long borders = ((long long)n - 1) / len;
+  int across = 16;
+  while (across < EMB_JOIN_THREADS && across < width) across *= 2;
   if (borders > 0)
-    hipLaunchKernelGGL((emb_join<T>), dim3((unsigned)borders), dim3(EMB_THREADS), 0, s, n, (uint32_t)vocab, width,
-                       w.keys[side], scale, w.slots, (T*)dweight);
+    hipLaunchKernelGGL((emb_join<T>), dim3((unsigned)borders), dim3(EMB_JOIN_THREADS), 0, s, n, (uint32_t)vocab, width, across,
+                       len, w.keys[side], scale, w.slots, (T*)dweight);
+}
+
+template <typename T, typename ID, int W>
+void emb_few_launch(const EmbFew& f, long long n, int vocab, int width, const void* ids, long long padding, const void* dy,
+                    float scale, void* dweight, float* part, hipStream_t s) {
+  const size_t lds = (size_t)vocab * EMB_THREADS * W * 4;
+  hipLaunchKernelGGL((emb_few<T, ID, W>), dim3(f.blocks, f.slabs), dim3(EMB_THREADS), lds, s, n, vocab, width, f.lanes,
+                     f.share, (const ID*)ids, padding, (const T*)dy, part);
+  const int cells = vocab * width;
+  hipLaunchKernelGGL((emb_few_join<T>), dim3((cells + EMB_SUM_CELLS - 1) / EMB_SUM_CELLS), dim3(EMB_SUM_THREADS), 0, s, cells,
+                     f.blocks, part, scale, (T*)dweight);
 }
 
 template <typename ID>
@@ -379,10 +527,22 @@ int emb_sort(int n, long long vocab, const ID* ids, long long padding, const Emb
 template <typename T>
 void emb_backward_typed(int n, long long vocab, int width, const void* ids, int ids_bytes, const void* dy, float scale,
                         long long padding, void* dweight, const EmbSpace& w, hipStream_t s) {
+  const EmbFew f = emb_few_plan(n, vocab, width, sizeof(T));
+  if (f.use && (uintptr_t)dy % (f.words * sizeof(T)) == 0) {
+    float* part = (float*)w.keys[0];
+    if (ids_bytes == 4) {
+      if constexpr (sizeof(T) == 2)
+        if (f.words == 2) return emb_few_launch<T, int, 2>(f, n, (int)vocab, width, ids, padding, dy, scale, dweight, part, s);
+      return emb_few_launch<T, int, 1>(f, n, (int)vocab, width, ids, padding, dy, scale, dweight, part, s);
+    }
+    if constexpr (sizeof(T) == 2)
+      if (f.words == 2) return emb_few_launch<T, long long, 2>(f, n, (int)vocab, width, ids, padding, dy, scale, dweight, part, s);
+    return emb_few_launch<T, long long, 1>(f, n, (int)vocab, width, ids, padding, dy, scale, dweight, part, s);
+  }
   const long long cells = vocab * width;
   hipLaunchKernelGGL((emb_zero<T>), dim3((unsigned)std::min((cells + EMB_THREADS - 1) / EMB_THREADS, 8192LL)),
                      dim3(EMB_THREADS), 0, s, cells, (T*)dweight);
-  if (n == 0) return;
+  if (n == 0) return;  // (all rows are zero)
   const int side = ids_bytes == 4 ? emb_sort<int>(n, vocab, (const int*)ids, padding, w, s)
                                   : emb_sort<long long>(n, vocab, (const long long*)ids, padding, w, s);
   const int v = emb_vector(width, sizeof(T), (uintptr_t)dy | (uintptr_t)dweight);
@@ -414,10 +574,10 @@ extern "C" NSA_API int nsa_embedding_forward(long long tokens, long long vocab, 
 }
 
 extern "C" NSA_API size_t nsa_embedding_workspace(long long tokens, long long vocab, int width, int dtype) {
-  (void)vocab;
-  (void)dtype;
-  if (tokens <= 0 || width <= 0) return 0;
-  return emb_space(nullptr, tokens, width).bytes;
+  if (tokens <= 0 || vocab <= 0 || width <= 0 || !nsa_elem_known(dtype)) return 0;
+  const EmbFew f = emb_few_plan(tokens, vocab, width, nsa_elem_bytes(dtype));
+  const size_t few = f.use ? (size_t)f.blocks * vocab * width * sizeof(float) : 0;
+  return std::max(few, emb_space(nullptr, tokens, width).bytes);
 }
 
 extern "C" NSA_API int nsa_embedding_backward(long long tokens, long long vocab, int width, int dtype, const void* ids_dev,

@@ -16,7 +16,7 @@
 
 #include "nsa_elem.h"
 
-#define NG_RUNS 160          // runs per launch: 2 x 8 bytes each, inside the 4 KB of a kernel's arguments
+#define NG_RUNS 224          // runs per launch: 2 x 8 bytes each, inside the 4 KB of a kernel's arguments
 #define NG_THREADS 256
 #define NG_BLOCKS 2048       // workgroups of a launch at most: 8 per compute unit ...
 #define NG_BLOCKS_MIN 128    // ... and fewer where there are many launches: every partial sum is read by all of them
@@ -31,35 +31,35 @@ struct NgRuns {
 // |a| and |b| -> the larger one, NaN if either is one (fmaxf drops it)
 __device__ __forceinline__ float ng_max(float a, float b) { return (a > b || a != a) ? a : b; }
 
+// Four running sums: neighbouring elements go to different ones, so that no 64-bit addition waits for the one before it.
 template <int KIND>
 struct NgAcc {
-  double s = 0.0;
-  __device__ __forceinline__ void add(float v) {
-    if constexpr (KIND == NSA_NORM_L2) s = fma((double)v, (double)v, s);
-    else if constexpr (KIND == NSA_NORM_L1) s += (double)fabsf(v);
-    else s = (double)ng_max((float)s, fabsf(v));
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
+  __device__ __forceinline__ void add(float v, int i) {
+    double& a = s[i & 3];
+    if constexpr (KIND == NSA_NORM_L2) a = fma((double)v, (double)v, a);
+    else if constexpr (KIND == NSA_NORM_L1) a += (double)fabsf(v);
+    else a = (double)ng_max((float)a, fabsf(v));
   }
-  __device__ __forceinline__ void join(double o) {
-    if constexpr (KIND == NSA_NORM_INF) s = (s > o || s != s) ? s : o;
-    else s += o;
+  static __device__ __forceinline__ double two(double a, double b) {
+    if constexpr (KIND == NSA_NORM_INF) return (a > b || a != a) ? a : b;
+    else return a + b;
   }
+  __device__ __forceinline__ double all() const { return two(two(s[0], s[1]), two(s[2], s[3])); }
 };
 
 template <int KIND, int THREADS>
 __device__ __forceinline__ double ng_block_join(double s) {  // the sum on every thread, in a fixed order
   __shared__ double part[THREADS / 64];
-  NgAcc<KIND> a;
-  a.s = s;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) a.join(__shfl_xor(a.s, o));
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = a.s;
+  for (int o = 32; o > 0; o >>= 1) s = NgAcc<KIND>::two(s, __shfl_xor(s, o));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
-  NgAcc<KIND> all;
-  all.s = part[0];
+  s = part[0];
 #pragma unroll
-  for (int w = 1; w < THREADS / 64; ++w) all.join(part[w]);
+  for (int w = 1; w < THREADS / 64; ++w) s = NgAcc<KIND>::two(s, part[w]);
   __syncthreads();
-  return all.s;
+  return s;
 }
 
 // the elements [lo, hi) of the launch, run by run: f(pointer, length), each a contiguous piece
@@ -79,24 +79,55 @@ __device__ __forceinline__ void ng_pieces(const NgRuns& r, long long lo, long lo
   }
 }
 
+// One contiguous piece, cut into single elements up to the first 16-byte border, accesses of 16 bytes - NG_AHEAD of them
+// asked for before the first is used - and single elements behind the last border.
+//   one(pointer): a single element;  wide(pointer, count): `count` accesses, NG_THREADS of them apart
+#define NG_AHEAD 4
+template <typename T, typename ONE, typename WIDE>
+__device__ __forceinline__ void ng_piece(T* p, long long len, ONE one, WIDE wide) {
+  constexpr int V = 16 / sizeof(T);
+  long long head = (16 - ((uintptr_t)p & 15)) & 15;
+  head = head / (long long)sizeof(T) < len ? head / (long long)sizeof(T) : len;
+  const long long body = (len - head) / V * V;
+  if (threadIdx.x < head) one(p + threadIdx.x);
+  T* q = p + head;
+  long long i = (long long)threadIdx.x * V;
+  for (; i + (NG_AHEAD - 1) * NG_THREADS * V < body; i += NG_AHEAD * NG_THREADS * V) wide(q + i, NG_AHEAD);
+  for (; i < body; i += NG_THREADS * V) wide(q + i, 1);
+  const long long rest = len - head - body;  // fewer than V
+  if (threadIdx.x < rest) one(q + body + threadIdx.x);
+}
+
 template <typename T, int KIND>
 __global__ void __launch_bounds__(NG_THREADS) ng_partial(NgRuns r, long long share, double* __restrict__ partial) {
+  constexpr int V = 16 / sizeof(T);
   NgAcc<KIND> acc;
   const long long lo = blockIdx.x * share;
   const long long hi = lo + share < r.first[r.count] ? lo + share : r.first[r.count];
   ng_pieces(r, lo, hi, [&](const void* base, long long at, long long len) {
-    const T* p = (const T*)base + at;
-    for (long long i = threadIdx.x; i < len; i += NG_THREADS) acc.add((float)p[i]);
+    ng_piece((const T*)base + at, len, [&](const T* p) { acc.add((float)*p, 0); },
+             [&](const T* p, int count) {
+               float v[NG_AHEAD][V];
+#pragma unroll
+               for (int k = 0; k < NG_AHEAD; ++k)
+                 if (k < count) nsa_load<T, V>(p + k * NG_THREADS * V, v[k]);
+#pragma unroll
+               for (int k = 0; k < NG_AHEAD; ++k)
+                 if (k < count) {
+#pragma unroll
+                   for (int i = 0; i < V; ++i) acc.add(v[k][i], i);
+                 }
+             });
   });
-  const double s = ng_block_join<KIND, NG_THREADS>(acc.s);
+  const double s = ng_block_join<KIND, NG_THREADS>(acc.all());
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
 template <int KIND>
 __device__ __forceinline__ float ng_total(const double* __restrict__ partial, int n_partial) {
-  NgAcc<KIND> acc;
-  for (int i = threadIdx.x; i < n_partial; i += NG_THREADS) acc.join(partial[i]);
-  const double s = ng_block_join<KIND, NG_THREADS>(acc.s);
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n_partial; i += NG_THREADS) s = NgAcc<KIND>::two(s, partial[i]);
+  s = ng_block_join<KIND, NG_THREADS>(s);
   return (float)(KIND == NSA_NORM_L2 ? sqrt(s) : s);
 }
 
@@ -118,16 +149,76 @@ __device__ __forceinline__ float ng_factor(float norm, float max_norm) {
 template <typename T, int KIND>
 __global__ void __launch_bounds__(NG_THREADS) ng_scale(NgRuns r, long long share, const double* __restrict__ partial,
                                                        int n_partial, float max_norm, float* __restrict__ norm_out) {
+  constexpr int V = 16 / sizeof(T);
   const float norm = ng_total<KIND>(partial, n_partial);
   if (blockIdx.x == 0 && threadIdx.x == 0 && norm_out != nullptr) norm_out[0] = norm;
   const float f = ng_factor(norm, max_norm);
   if (f == 1.0f) return;  // (a product by one changes nothing)
-  const long long lo = blockIdx.x * share;
+  // the shares from the last to the first: what the norm read last is the likeliest to be in a cache still
+  const long long lo = (gridDim.x - 1 - blockIdx.x) * share;
   const long long hi = lo + share < r.first[r.count] ? lo + share : r.first[r.count];
   ng_pieces(r, lo, hi, [&](void* base, long long at, long long len) {
-    T* p = (T*)base + at;
-    for (long long i = threadIdx.x; i < len; i += NG_THREADS) p[i] = (T)((float)p[i] * f);
+    ng_piece((T*)base + at, len, [&](T* p) { *p = (T)((float)*p * f); },
+             [&](T* p, int count) {
+               float v[NG_AHEAD][V];
+#pragma unroll
+               for (int k = 0; k < NG_AHEAD; ++k)
+                 if (k < count) nsa_load<T, V>(p + k * NG_THREADS * V, v[k]);
+#pragma unroll
+               for (int k = 0; k < NG_AHEAD; ++k)
+                 if (k < count) {
+#pragma unroll
+                   for (int i = 0; i < V; ++i) v[k][i] *= f;
+                   nsa_store<T, V>(p + k * NG_THREADS * V, v[k]);
+                 }
+             });
   });
+}
+
+// A few thousand elements: norm and clip in one workgroup and one launch, each element kept in a register between
+// them.  (Two launches cost their start twice; beyond NG_SMALL elements one compute unit is slower than that.)
+#define NG_SMALL_THREADS 1024
+#define NG_SMALL_EACH 16
+#define NG_SMALL (NG_SMALL_THREADS * NG_SMALL_EACH)
+template <typename T, int KIND>
+__global__ void __launch_bounds__(NG_SMALL_THREADS) ng_small(NgRuns r, int clip, float max_norm,
+                                                             float* __restrict__ norm_out) {
+  __shared__ int first[NG_RUNS + 1];
+  __shared__ T* ptr[NG_RUNS];
+  for (int k = threadIdx.x; k <= r.count; k += NG_SMALL_THREADS) {
+    first[k] = (int)r.first[k];
+    if (k < r.count) ptr[k] = (T*)r.ptr[k];
+  }
+  __syncthreads();
+  const int total = first[r.count];
+  T* at[NG_SMALL_EACH];
+  float v[NG_SMALL_EACH];
+#pragma unroll
+  for (int k = 0; k < NG_SMALL_EACH; ++k) {
+    const int e = k * NG_SMALL_THREADS + threadIdx.x;
+    v[k] = 0.0f;
+    if (e < total) {
+      int a = 0, b = r.count;
+      while (b - a > 1) {
+        const int m = (a + b) >> 1;
+        if (first[m] <= e) a = m;
+        else b = m;
+      }
+      at[k] = ptr[a] + (e - first[a]);
+      v[k] = (float)*at[k];
+    }
+  }
+  NgAcc<KIND> acc;
+#pragma unroll
+  for (int k = 0; k < NG_SMALL_EACH; ++k) acc.add(v[k], k);
+  const double s = ng_block_join<KIND, NG_SMALL_THREADS>(acc.all());
+  const float norm = (float)(KIND == NSA_NORM_L2 ? sqrt(s) : s);
+  if (threadIdx.x == 0) norm_out[0] = norm;
+  const float f = clip ? ng_factor(norm, max_norm) : 1.0f;
+  if (f == 1.0f) return;
+#pragma unroll
+  for (int k = 0; k < NG_SMALL_EACH; ++k)
+    if (k * NG_SMALL_THREADS + (int)threadIdx.x < total) *at[k] = (T)(v[k] * f);
 }
 
 // ---------------------------------------------------------------------------
@@ -230,6 +321,12 @@ int ng_run(const char* what, int count, void* const* tensors, const long long* s
     const bool apart = ng_runs(count, tensors, sizes, dtypes, runs);
     if (clip && !apart) return nsa_fail(NSA_E_ARG, "%s: two gradients overlap in memory", what);
     ng_launches(runs, launches);
+    if (launches.size() == 1 && launches[0].r.first[launches[0].r.count] <= NG_SMALL) {
+      const Launch& l = launches[0];
+      NG_DISPATCH(l.dtype, ng_small, dim3(1), dim3(NG_SMALL_THREADS), 0, s, l.r, clip ? 1 : 0, max_norm, norm_out)
+      const hipError_t e = hipGetLastError();
+      return e == hipSuccess ? NSA_OK : nsa_fail(NSA_E_HIP, "%s: %s", what, hipGetErrorString(e));
+    }
     int n_partial = 0;
     for (const Launch& l : launches) {
       NG_DISPATCH(l.dtype, ng_partial, dim3(l.blocks), dim3(NG_THREADS), 0, s, l.r, l.share, workspace + n_partial)

@@ -24,12 +24,23 @@
 // activations
 // ---------------------------------------------------------------------------
 
-__device__ __forceinline__ float gn_sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
+// 1 / (1 + e^-z) by the hardware's 2^x and reciprocal (1 ulp each; the product z log2(e) adds |z| ulp, where e^-z decides)
+__device__ __forceinline__ float gn_sigmoid(float z) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z));
+}
+
+// 2 / (1 + e^-2z) - 1; near zero, where that is a difference of equal numbers, the series z - z^3/3 + 2 z^5/15 - 17 z^7/315
+// (the next term is 62 z^9 / 2835: below 2^-28 of z at the border)
+__device__ __forceinline__ float gn_tanh(float z) {
+  const float s = z * z;
+  const float near = z * fmaf(s, fmaf(s, fmaf(s, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+  return fabsf(z) < 0.15f ? near : fmaf(2.0f, gn_sigmoid(2.0f * z), -1.0f);
+}
 
 template <int ACT>
 __device__ __forceinline__ float gn_act(float z) {
   if constexpr (ACT == NSA_FN_RELU) return z < 0.0f ? 0.0f : z;  // (NaN stays)
-  else if constexpr (ACT == NSA_FN_TANH) return tanhf(z);
+  else if constexpr (ACT == NSA_FN_TANH) return gn_tanh(z);
   else if constexpr (ACT == NSA_FN_SILU) return z * gn_sigmoid(z);
   else return z;
 }
@@ -37,12 +48,12 @@ __device__ __forceinline__ float gn_act(float z) {
 template <int ACT>
 __device__ __forceinline__ float gn_slope(float z) {
   if constexpr (ACT == NSA_FN_RELU) return z > 0.0f ? 1.0f : 0.0f;
-  else if constexpr (ACT == NSA_FN_TANH) {
-    const float t = tanhf(z);
-    return 1.0f - t * t;
+  else if constexpr (ACT == NSA_FN_TANH) {  // 1 - tanh^2 = 4 s (1 - s) with s = sigmoid(2 z)
+    const float s = gn_sigmoid(2.0f * z);
+    return 4.0f * s * (1.0f - s);
   } else if constexpr (ACT == NSA_FN_SILU) {
     const float s = gn_sigmoid(z);
-    return s * (1.0f + z * (1.0f - s));
+    return s * fmaf(z, 1.0f - s, 1.0f);
   } else return 1.0f;
 }
 
@@ -342,35 +353,273 @@ __global__ void __launch_bounds__(GN_THREADS) gn_dx(GnShape s, const T* __restri
   }
 }
 
-// The parameters' gradients: `count` records of [channels] sums, `stride` apart, added in a fixed order.  A workgroup per 64
-// channels, four waves that take every fourth record each.
+// The parameters' gradients: `count` records of [channels] sums, `stride` apart, added in 64 bits (there may be as many
+// records as samples) and a fixed order.  A workgroup per GN_PARAM_CH channels; its threads share the records out.
+#define GN_PARAM_THREADS 1024
+#define GN_PARAM_CH 16
 template <typename T>
-__global__ void __launch_bounds__(GN_THREADS) gn_param_grads(int channels, long long count, long long stride,
-                                                             const float2* __restrict__ part, int f32,
-                                                             void* __restrict__ dw, void* __restrict__ db) {
-  __shared__ float2 red[GN_THREADS];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
-  float2 t = make_float2(0.0f, 0.0f);
-  if (c < channels)
-    for (long long k = wave; k < count; k += GN_THREADS / 64) {
-      const float2 o = part[k * stride + c];
-      t.x += o.x;
-      t.y += o.y;
+__global__ void __launch_bounds__(GN_PARAM_THREADS) gn_param_grads(int channels, long long count, long long stride,
+                                                                   const float2* __restrict__ part, int f32,
+                                                                   void* __restrict__ dw, void* __restrict__ db) {
+  constexpr int LANES = GN_PARAM_THREADS / GN_PARAM_CH;
+  __shared__ double2 red[GN_PARAM_THREADS];
+  const int c = blockIdx.x * GN_PARAM_CH + threadIdx.x % GN_PARAM_CH;
+  const int lane = threadIdx.x / GN_PARAM_CH;
+  double2 t = make_double2(0.0, 0.0);
+  if (c < channels) {
+    const float2* p = part + c;
+#pragma unroll 4
+    for (long long k = lane; k < count; k += LANES) {
+      const float2 o = p[k * stride];
+      t.x += (double)o.x;
+      t.y += (double)o.y;
     }
+  }
   red[threadIdx.x] = t;
   __syncthreads();
-  if (wave != 0 || c >= channels) return;
-  for (int w = 1; w < GN_THREADS / 64; ++w) {
-    t.x += red[w * 64 + threadIdx.x].x;
-    t.y += red[w * 64 + threadIdx.x].y;
+#pragma unroll
+  for (int half = LANES / 2; half > 0; half >>= 1) {
+    if (lane < half) {
+      red[threadIdx.x].x += red[threadIdx.x + half * GN_PARAM_CH].x;
+      red[threadIdx.x].y += red[threadIdx.x + half * GN_PARAM_CH].y;
+    }
+    __syncthreads();
   }
+  if (lane != 0 || c >= channels) return;
+  t = red[threadIdx.x];
   if (f32) {
-    if (dw != nullptr) ((float*)dw)[c] = t.y;
-    if (db != nullptr) ((float*)db)[c] = t.x;
+    if (dw != nullptr) ((float*)dw)[c] = (float)t.y;
+    if (db != nullptr) ((float*)db)[c] = (float)t.x;
   } else {
-    if (dw != nullptr) ((T*)dw)[c] = (T)t.y;
-    if (db != nullptr) ((T*)db)[c] = (T)t.x;
+    if (dw != nullptr) ((T*)dw)[c] = (T)(float)t.y;
+    if (db != nullptr) ((T*)db)[c] = (T)(float)t.x;
   }
+}
+
+// ---------------------------------------------------------------------------
+// small samples: whole samples in one workgroup, each value read once
+// ---------------------------------------------------------------------------
+
+// A tile of `per` whole samples, at most THREADS * GN_EACH values, contiguous in memory.  Its values go through LDS in
+// float32: a team of `team` lanes takes a (sample, group), whose channels may lie anywhere in a thread's accesses.
+#define GN_EACH 16
+struct GnTile {
+  long long samples;
+  int length, channels, groups, cpg;
+  int values;                 // of a sample: length * channels
+  int per;                    // samples of a tile
+  int team, step_l, step_c;   // lanes per (sample, group); `team` values on = step_l positions and step_c channels on
+  uint32_t by_values, by_channels, by_cpg;  // 2^32 / d + 1 (0: d = 1): quotients of numbers up to 2^14 by d up to 2^14
+  int fixed;                  // a thread's accesses all lie in the same channels
+};
+
+__device__ __forceinline__ int gn_div(int n, uint32_t by) { return by != 0 ? (int)__umulhi((uint32_t)n, by) : n; }
+
+// f(value index in the tile) over the values of group g of sample s, lane by lane of its team
+template <typename F>
+__device__ __forceinline__ void gn_walk(const GnTile& q, int s, int g, int lane, F f) {
+  int l = gn_div(lane, q.by_cpg), c = lane - l * q.cpg;
+  int at = s * q.values + l * q.channels + g * q.cpg + c;
+  const int step = q.step_l * q.channels + q.step_c, wrap = q.channels - q.cpg;
+  while (l < q.length) {
+    f(at, g * q.cpg + c);
+    l += q.step_l;
+    c += q.step_c;
+    at += step;
+    if (c >= q.cpg) {
+      c -= q.cpg;
+      ++l;
+      at += wrap;
+    }
+  }
+}
+
+__device__ __forceinline__ float gn_team_sum(float a, int team) {
+  for (int o = team >> 1; o > 0; o >>= 1) a += __shfl_xor(a, o);
+  return a;
+}
+
+// group, weight and bias of the V channels at value e of a tile
+template <typename T, int V>
+__device__ __forceinline__ void gn_channels(const GnTile& q, const GnParams& par, int e, int (&g)[V], float (&w)[V],
+                                            float (&b)[V]) {
+  const int c = e - gn_div(e, q.by_channels) * q.channels;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    g[i] = gn_div(c + i, q.by_cpg);
+    w[i] = gn_param<T>(par.w, par.f32, c + i, 1.0f);
+    b[i] = gn_param<T>(par.b, par.f32, c + i, 0.0f);
+  }
+}
+
+template <typename T, int V, int ACT, int THREADS>
+__global__ void __launch_bounds__(THREADS) gn_tile_forward(GnTile q, const T* __restrict__ x, GnParams par, float eps,
+                                                           float* __restrict__ mean, float* __restrict__ rstd,
+                                                           T* __restrict__ y) {
+  constexpr int STEPS = GN_EACH / V;
+  extern __shared__ float lds[];
+  float* buf = lds;                                    // [THREADS * GN_EACH]
+  float2* stat = (float2*)(lds + THREADS * GN_EACH);   // [per * groups]
+  const long long first = (long long)blockIdx.x * q.per;
+  const int here = q.samples - first < q.per ? (int)(q.samples - first) : q.per;
+  const int values = here * q.values;
+  const long long base = first * q.values;
+  float v[STEPS][V];
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) {
+    const int e = (k * THREADS + threadIdx.x) * V;
+    if (e < values) nsa_load<T, V>(x + base + e, v[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) {
+    const int e = (k * THREADS + threadIdx.x) * V;
+    if (e < values) nsa_store<float, V>(buf + e, v[k]);
+  }
+  __syncthreads();
+  const int pairs = here * q.groups, lane = threadIdx.x & (q.team - 1);
+  const float m = (float)q.length * (float)q.cpg;
+  for (int p = threadIdx.x / q.team; p < pairs; p += THREADS / q.team) {
+    const int s = p / q.groups, g = p - s * q.groups;
+    const float shift = buf[s * q.values + g * q.cpg];
+    float a = 0.0f;
+    gn_walk(q, s, g, lane, [&](int at, int) { a += buf[at] - shift; });
+    const float mu = shift + gn_team_sum(a, q.team) / m;
+    float b = 0.0f;
+    gn_walk(q, s, g, lane, [&](int at, int) {
+      const float d = buf[at] - mu;
+      b = fmaf(d, d, b);
+    });
+    const float rs = 1.0f / sqrtf(gn_team_sum(b, q.team) / m + eps);
+    if (lane == 0) {
+      stat[p] = make_float2(mu, rs);
+      mean[first * q.groups + p] = mu;
+      rstd[first * q.groups + p] = rs;
+    }
+  }
+  __syncthreads();
+  float w[V], b[V];
+  int g[V];
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) {
+    const int e = (k * THREADS + threadIdx.x) * V;
+    if (e >= values) continue;
+    const int s = gn_div(e, q.by_values);
+    if (k == 0 || !q.fixed) gn_channels<T, V>(q, par, e, g, w, b);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float2 t = stat[s * q.groups + g[i]];
+      v[k][i] = gn_act<ACT>(fmaf((v[k][i] - t.x) * t.y, w[i], b[i]));
+    }
+    nsa_store<T, V>(y + base + e, v[k]);
+  }
+}
+
+// The same tiles backward: dz and dz xh through LDS, from which the teams take A and B and the threads the columns' sums
+// for the parameters.  A workgroup walks over tiles, keeps the columns' sums in LDS and writes one record of them at the end:
+// part[block][channels].
+template <typename T, int V, int ACT, int THREADS>
+__global__ void __launch_bounds__(THREADS) gn_tile_backward(GnTile q, const T* __restrict__ x, const T* __restrict__ dy,
+                                                            GnParams par, const float* __restrict__ mean,
+                                                            const float* __restrict__ rstd, T* __restrict__ dx,
+                                                            float2* __restrict__ part) {
+  constexpr int STEPS = GN_EACH / V;
+  extern __shared__ float lds[];
+  float* bz = lds;                                            // [THREADS * GN_EACH]  dz
+  float* bzx = lds + THREADS * GN_EACH;                       //                      dz xh
+  float2* ab = (float2*)(lds + 2 * THREADS * GN_EACH);        // [per * groups]
+  float* bw = (float*)(ab + q.per * q.groups);                // [channels] weights
+  float2* cols = (float2*)(bw + (q.channels + 1) / 2 * 2);    // [subs][channels]
+  const int subs = q.channels < THREADS ? THREADS / q.channels : 1;
+  for (int c = threadIdx.x; c < q.channels; c += THREADS) bw[c] = gn_param<T>(par.w, par.f32, c, 1.0f);
+  for (int i = threadIdx.x; i < subs * q.channels; i += THREADS) cols[i] = make_float2(0.0f, 0.0f);
+  const float m = (float)q.length * (float)q.cpg;
+  const long long tiles = (q.samples + q.per - 1) / q.per;
+  __syncthreads();
+  for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const long long first = tile * q.per, base = first * q.values;
+    const int here = q.samples - first < q.per ? (int)(q.samples - first) : q.per;
+    const int values = here * q.values;
+    float v[STEPS][V], z[STEPS][V], w[V], b[V];
+    int g[V];
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {
+      const int e = (k * THREADS + threadIdx.x) * V;
+      if (e < values) {
+        nsa_load<T, V>(x + base + e, v[k]);
+        nsa_load<T, V>(dy + base + e, z[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {
+      const int e = (k * THREADS + threadIdx.x) * V;
+      if (e >= values) continue;
+      const long long p = (first + gn_div(e, q.by_values)) * q.groups;
+      if (k == 0 || !q.fixed) gn_channels<T, V>(q, par, e, g, w, b);
+      float zx[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        v[k][i] = (v[k][i] - mean[p + g[i]]) * rstd[p + g[i]];
+        z[k][i] *= gn_slope<ACT>(fmaf(v[k][i], w[i], b[i]));
+        zx[i] = z[k][i] * v[k][i];
+      }
+      nsa_store<float, V>(bz + e, z[k]);
+      nsa_store<float, V>(bzx + e, zx);
+    }
+    __syncthreads();
+    const int pairs = here * q.groups, lane = threadIdx.x & (q.team - 1);
+    if (dx != nullptr)
+      for (int p = threadIdx.x / q.team; p < pairs; p += THREADS / q.team) {
+        const int s = p / q.groups, g = p - s * q.groups;
+        float a = 0.0f, b = 0.0f;
+        gn_walk(q, s, g, lane, [&](int at, int c) {
+          a = fmaf(bw[c], bz[at], a);
+          b = fmaf(bw[c], bzx[at], b);
+        });
+        a = gn_team_sum(a, q.team);
+        b = gn_team_sum(b, q.team);
+        if (lane == 0) ab[p] = make_float2(a / m, b / m);
+      }
+    if (part != nullptr) {
+      const int rows = here * q.length;
+      for (int i = threadIdx.x; i < subs * q.channels; i += THREADS) {
+        const int sub = i / q.channels, c = i - sub * q.channels;
+        float2 t = make_float2(0.0f, 0.0f);
+        for (int r = sub; r < rows; r += subs) {
+          t.x += bz[r * q.channels + c];
+          t.y += bzx[r * q.channels + c];
+        }
+        cols[i].x += t.x;
+        cols[i].y += t.y;
+      }
+    }
+    __syncthreads();
+    if (dx != nullptr) {
+#pragma unroll
+      for (int k = 0; k < STEPS; ++k) {
+        const int e = (k * THREADS + threadIdx.x) * V;
+        if (e >= values) continue;
+        const int s = gn_div(e, q.by_values);
+        if (!q.fixed) gn_channels<T, V>(q, par, e, g, w, b);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float2 t = ab[s * q.groups + g[i]];
+          z[k][i] = rstd[(first + s) * q.groups + g[i]] * (w[i] * z[k][i] - t.x - v[k][i] * t.y);
+        }
+        nsa_store<T, V>(dx + base + e, z[k]);
+      }
+    }
+    // (the next tile's dz is written to LDS by threads that have passed the barrier above: nothing reads the old one)
+  }
+  __syncthreads();
+  if (part != nullptr)
+    for (int c = threadIdx.x; c < q.channels; c += THREADS) {
+      float2 t = cols[c];
+      for (int s = 1; s < subs; ++s) {
+        t.x += cols[s * q.channels + c].x;
+        t.y += cols[s * q.channels + c].y;
+      }
+      part[(long long)blockIdx.x * q.channels + c] = t;
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -415,6 +664,32 @@ GnShape gn_shape(long long samples, long long length, int channels, int groups, 
   return s;
 }
 
+const size_t GN_LDS = 152 * 1024;  // of a workgroup's 160 KB
+const int GN_TILE_BLOCKS = 1024;  // workgroups of the backward tiles: one record of column sums each
+
+bool gn_tile(long long samples, long long length, int channels, int groups, int v, int most, GnTile& q) {
+  if (length * channels > most) return false;
+  q.samples = samples;
+  q.length = (int)length;
+  q.channels = channels;
+  q.groups = groups;
+  q.cpg = channels / groups;
+  q.values = q.length * channels;
+  q.per = most / q.values;
+  // (accesses of v values must not run over a tile's end, and samples begin at multiples of v: channels is one)
+  const int threads = most / GN_EACH, group = q.length * q.cpg;
+  q.team = 1;
+  while (q.team < 64 && q.team * 2 <= group && q.per * groups * q.team < threads) q.team *= 2;
+  q.step_l = q.team / q.cpg;
+  q.step_c = q.team % q.cpg;
+  q.fixed = threads * v % channels == 0;
+  auto by = [](int d) { return d == 1 ? 0u : (uint32_t)((1ULL << 32) / d + 1); };
+  q.by_values = by(q.values);
+  q.by_channels = by(channels);
+  q.by_cpg = by(q.cpg);
+  return true;
+}
+
 // An upper bound that does not ask for the addresses: chunks do not grow with a narrower access by more than the rows do
 size_t gn_workspace(long long samples, long long length, int channels, int groups, int bytes, bool backward) {
   size_t most = 0;
@@ -424,6 +699,8 @@ size_t gn_workspace(long long samples, long long length, int channels, int group
     const size_t parts = (size_t)s.samples * s.chunks * (backward ? s.channels : s.groups) * sizeof(float2);
     most = std::max(most, parts);
   }
+  if (backward && length * channels <= 256 * GN_EACH)  // the tiles' records
+    most = std::max(most, (size_t)std::min(samples, (long long)GN_TILE_BLOCKS) * channels * sizeof(float2));
   return most + (backward ? (size_t)samples * groups * sizeof(float2) : 0) + 256;
 }
 
@@ -444,6 +721,20 @@ int gn_done(const char* what) {
   return e == hipSuccess ? NSA_OK : nsa_fail(NSA_E_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 
+// a launch with more dynamic LDS than the 64 KB that need no asking
+#define GN_TILE_LAUNCH(KERNEL, lds, ...)                                                                                  \
+  {                                                                                                                       \
+    if ((lds) > 64 * 1024)                                                                                                \
+      (void)hipFuncSetAttribute((const void*)(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, (int)(lds));           \
+    hipLaunchKernelGGL((KERNEL), __VA_ARGS__);                                                                            \
+  }
+#define GN_TILE_ACTS(act, KERNEL, T, V, THREADS, lds, ...)                                                                \
+  switch (act) {                                                                                                          \
+    case NSA_FN_RELU: GN_TILE_LAUNCH((KERNEL<T, V, NSA_FN_RELU, THREADS>), lds, __VA_ARGS__) break;                       \
+    case NSA_FN_TANH: GN_TILE_LAUNCH((KERNEL<T, V, NSA_FN_TANH, THREADS>), lds, __VA_ARGS__) break;                       \
+    case NSA_FN_SILU: GN_TILE_LAUNCH((KERNEL<T, V, NSA_FN_SILU, THREADS>), lds, __VA_ARGS__) break;                       \
+    default: GN_TILE_LAUNCH((KERNEL<T, V, NSA_FN_NONE, THREADS>), lds, __VA_ARGS__) break;                                \
+  }
 #define GN_ACTS(act, KERNEL, T, V, ...)                                                             \
   switch (act) {                                                                                    \
     case NSA_FN_RELU: hipLaunchKernelGGL((KERNEL<T, V, NSA_FN_RELU>), __VA_ARGS__); break;          \
@@ -455,6 +746,19 @@ int gn_done(const char* what) {
 template <typename T, int V>
 void gn_forward(const GnShape& s, const void* x, GnParams q, float eps, int act, void* y, float* mean, float* rstd,
                 float2* part, hipStream_t st) {
+  GnTile q_;
+  for (int threads = 256; threads <= 1024; threads *= 4) {
+    if (!gn_tile(s.samples, s.length, s.channels, s.groups, V, threads * GN_EACH, q_)) continue;
+    const size_t lds = (size_t)threads * GN_EACH * 4 + (size_t)q_.per * q_.groups * sizeof(float2);
+    if (lds > GN_LDS) break;
+    const dim3 tiles((unsigned)((s.samples + q_.per - 1) / q_.per));
+    if (threads == 256) {
+      GN_TILE_ACTS(act, gn_tile_forward, T, V, 256, lds, tiles, dim3(256), lds, st, q_, (const T*)x, q, eps, mean, rstd, (T*)y)
+    } else {
+      GN_TILE_ACTS(act, gn_tile_forward, T, V, 1024, lds, tiles, dim3(1024), lds, st, q_, (const T*)x, q, eps, mean, rstd, (T*)y)
+    }
+    return;
+  }
   const dim3 grid((unsigned)(s.samples * s.slabs * s.chunks)), block(GN_THREADS);
   hipLaunchKernelGGL((gn_stats<T, V>), grid, block, 0, st, s, (const T*)x, part);
   const long long pairs = s.samples * s.groups;
@@ -466,6 +770,22 @@ void gn_forward(const GnShape& s, const void* x, GnParams q, float eps, int act,
 template <typename T, int V>
 void gn_backward(const GnShape& s, const void* x, const void* dy, GnParams q, int act, const float* mean, const float* rstd,
                  void* dx, void* dw, void* db, float2* part, float2* ab, hipStream_t st) {
+  GnTile q_;
+  if (gn_tile(s.samples, s.length, s.channels, s.groups, V, 256 * GN_EACH, q_)) {
+    const size_t lds = (size_t)256 * GN_EACH * 8 + (size_t)q_.per * q_.groups * sizeof(float2) +
+                       (size_t)(s.channels + 1) / 2 * 8 + (size_t)std::max(256, s.channels) * sizeof(float2);
+    if (lds <= GN_LDS) {
+      const bool sums = dw != nullptr || db != nullptr;
+      const int blocks = (int)std::min((s.samples + q_.per - 1) / q_.per, (long long)GN_TILE_BLOCKS);
+      GN_TILE_ACTS(act, gn_tile_backward, T, V, 256, lds, dim3(blocks), dim3(256), lds, st, q_, (const T*)x, (const T*)dy, q, mean,
+                   rstd, (T*)dx, sums ? part : nullptr)
+      if (sums)
+        hipLaunchKernelGGL((gn_param_grads<T>), dim3((unsigned)((s.channels + GN_PARAM_CH - 1) / GN_PARAM_CH)),
+                           dim3(GN_PARAM_THREADS), 0, st, s.channels, (long long)blocks, (long long)s.channels, part, q.f32,
+                           dw, db);
+      return;
+    }
+  }
   const dim3 grid((unsigned)(s.samples * s.slabs * s.chunks)), block(GN_THREADS);
   GN_ACTS(act, gn_sums, T, V, grid, block, 0, st, s, (const T*)x, (const T*)dy, q, mean, rstd, part)
   const long long pairs = s.samples * s.groups;
@@ -475,8 +795,9 @@ void gn_backward(const GnShape& s, const void* x, const void* dy, GnParams q, in
     GN_ACTS(act, gn_dx, T, V, grid, block, 0, st, s, (const T*)x, (const T*)dy, q, mean, rstd, ab, (T*)dx)
   }
   if (dw != nullptr || db != nullptr)
-    hipLaunchKernelGGL((gn_param_grads<T>), dim3((unsigned)((s.channels + 63) / 64)), block, 0, st, s.channels, s.samples,
-                       (long long)s.chunks * s.channels, part, q.f32, dw, db);
+    hipLaunchKernelGGL((gn_param_grads<T>), dim3((unsigned)((s.channels + GN_PARAM_CH - 1) / GN_PARAM_CH)),
+                       dim3(GN_PARAM_THREADS), 0, st, s.channels, s.samples, (long long)s.chunks * s.channels, part, q.f32, dw,
+                       db);
 }
 
 // one call per element type and access width
@@ -527,8 +848,8 @@ extern "C" NSA_API int nsa_group_norm_backward(long long samples, long long leng
   const int f32 = weight_dtype == NSA_DT_F32;
   if (samples == 0 || length == 0) {  // no rows: the parameters' gradients are zero
     if (dweight_dev == nullptr && dbias_dev == nullptr) return NSA_OK;
-    hipLaunchKernelGGL((gn_param_grads<nsa_f16>), dim3((unsigned)((channels + 63) / 64)), dim3(GN_THREADS), 0, st, channels,
-                       0LL, 0LL, (const float2*)nullptr, f32, dweight_dev, dbias_dev);  // (zero has the same bits in both 16-bit types)
+    hipLaunchKernelGGL((gn_param_grads<nsa_f16>), dim3((unsigned)((channels + GN_PARAM_CH - 1) / GN_PARAM_CH)),
+                       dim3(GN_PARAM_THREADS), 0, st, channels, 0LL, 0LL, (const float2*)nullptr, f32, dweight_dev, dbias_dev);  // (zero has the same bits in both 16-bit types)
     return gn_done(what);
   }
   if (!x_dev || !dy_dev || !mean_dev || !rstd_dev || !workspace_dev) return nsa_fail(NSA_E_ARG, "%s: NULL argument", what);
