@@ -15,9 +15,9 @@
 #include "nsa_elem.h"
 
 #define EMB_THREADS 256
-#define EMB_ITEMS 16                          // keys per thread of a sorting tile
-#define EMB_TILE (EMB_THREADS * EMB_ITEMS)
+#define EMB_MANY 400000                       // tokens from which a sorting tile has 16 keys per thread instead of 4
 #define EMB_AHEAD 8                           // rows in flight per team
+#define EMB_FEW_AHEAD 16                      // the same where a row is four bytes a lane
 #define EMB_FEW 64                            // rows of a table whose gradient is summed in LDS (64 KB)
 
 // ---------------------------------------------------------------------------
@@ -59,15 +59,16 @@ __device__ __forceinline__ uint32_t emb_key(const ID* ids, long long i, long lon
 }
 
 // digit counts of every tile: counts[digit][tile]; the first pass reads the ids themselves (keys == nullptr)
-template <typename ID>
+template <typename ID, int ITEMS>
 __global__ void __launch_bounds__(EMB_THREADS) emb_count(int n, const ID* __restrict__ ids, long long vocab,
                                                          long long padding, const uint32_t* __restrict__ keys, int shift,
                                                          uint32_t* __restrict__ counts) {
   __shared__ uint32_t bins[256];
   bins[threadIdx.x] = 0;
   __syncthreads();
-  const long long base = (long long)blockIdx.x * EMB_TILE;
-  for (int k = 0; k < EMB_ITEMS; ++k) {
+  const long long base = (long long)blockIdx.x * (EMB_THREADS * ITEMS);
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
     const long long i = base + k * EMB_THREADS + threadIdx.x;
     if (i < n) {
       const uint32_t key = keys != nullptr ? keys[i] : emb_key(ids, i, vocab, padding);
@@ -111,7 +112,7 @@ __global__ void __launch_bounds__(EMB_THREADS) emb_scan(int tiles, uint32_t* __r
 // The tile's keys to their places.  Each wave owns a contiguous quarter of the tile and counts its digits first; the place
 // of a key is then (keys of smaller digits) + (the digit's keys in earlier tiles, in earlier waves, in earlier rounds of
 // this wave, in lower lanes): equal digits keep their order.
-template <typename ID>
+template <typename ID, int ITEMS>
 __global__ void __launch_bounds__(EMB_THREADS) emb_scatter(int n, const ID* __restrict__ ids, long long vocab,
                                                            long long padding, const uint32_t* __restrict__ keys,
                                                            const uint32_t* __restrict__ pos, int shift,
@@ -136,10 +137,10 @@ __global__ void __launch_bounds__(EMB_THREADS) emb_scatter(int n, const ID* __re
   uint32_t first = s - total;
   for (int w = 0; w < wave; ++w) first += wave_sum[w];
 
-  const long long base = (long long)blockIdx.x * EMB_TILE + wave * (64 * EMB_ITEMS) + lane;
-  uint32_t key[EMB_ITEMS], from[EMB_ITEMS];
+  const long long base = (long long)blockIdx.x * (EMB_THREADS * ITEMS) + wave * (64 * ITEMS) + lane;
+  uint32_t key[ITEMS], from[ITEMS];
 #pragma unroll
-  for (int k = 0; k < EMB_ITEMS; ++k) {
+  for (int k = 0; k < ITEMS; ++k) {
     const long long i = base + k * 64;
     key[k] = from[k] = 0;
     if (i < n) {
@@ -157,7 +158,7 @@ __global__ void __launch_bounds__(EMB_THREADS) emb_scatter(int n, const ID* __re
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < EMB_ITEMS; ++k) {
+  for (int k = 0; k < ITEMS; ++k) {
     const bool here = base + k * 64 < n;
     const uint32_t digit = (key[k] >> shift) & 255u;
     unsigned long long same = __ballot(here);
@@ -182,21 +183,24 @@ __global__ void __launch_bounds__(EMB_THREADS) emb_scatter(int n, const ID* __re
 // sums over equal ids
 // ---------------------------------------------------------------------------
 
+// every row of the table, and the length of the list of runs
 template <typename T>
-__global__ void __launch_bounds__(EMB_THREADS) emb_zero(long long n, T* __restrict__ p) {
+__global__ void __launch_bounds__(EMB_THREADS) emb_zero(long long n, T* __restrict__ p, uint32_t* __restrict__ runs) {
+  if (blockIdx.x == 0 && threadIdx.x == 0 && runs != nullptr) runs[0] = 0;
   for (long long i = (long long)blockIdx.x * EMB_THREADS + threadIdx.x; i < n; i += (long long)gridDim.x * EMB_THREADS)
     p[i] = (T)0.0f;
 }
 
 // A team of `lanes` lanes takes a chunk of sorted positions, V columns to a lane; EMB_AHEAD rows are asked for before the first
 // is added.  slots[chunk][0]: the partial sum of an id that began in an earlier chunk; [1]: of one that began here and
-// goes on in the next.
+// goes on in the next: such a chunk is entered into the list `runs` (its length in runs[0]), in any order - the runs are
+// joined one by one.
 template <typename T, int V>
 __global__ void __launch_bounds__(EMB_THREADS) emb_reduce(int n, uint32_t vocab, int width, int lanes, int chunk_len,
                                                           const uint32_t* __restrict__ keys,
                                                           const uint32_t* __restrict__ pos, const T* __restrict__ dy,
                                                           float scale, T* __restrict__ dweight,
-                                                          float* __restrict__ slots) {
+                                                          float* __restrict__ slots, uint32_t* __restrict__ runs) {
   const int teams = EMB_THREADS / lanes;
   const long long chunk = (long long)blockIdx.x * teams + threadIdx.x / lanes;
   const long long begin = chunk * chunk_len;
@@ -245,41 +249,42 @@ __global__ void __launch_bounds__(EMB_THREADS) emb_reduce(int n, uint32_t vocab,
     }
   }
   leave(goes_on);
+  if (c == 0 && goes_on && !earlier && key != vocab) runs[1 + atomicAdd(runs, 1u)] = (uint32_t)chunk;
 }
 
-// One workgroup per chunk border: the id that goes over it is summed by the chunk in which it begins.  Long runs are shared by
-// the workgroup's parts, each a row of `lanes` threads; their sums are added in order.
-#define EMB_JOIN_THREADS 512
+// The runs over chunk borders, one by one: a workgroup takes EMB_JOIN_COLS columns of a run at a time; its four waves share
+// the run's chunks out and their sums are added in order.
+#define EMB_JOIN_COLS 64
 template <typename T>
-__global__ void __launch_bounds__(EMB_JOIN_THREADS) emb_join(int n, uint32_t vocab, int width, int lanes, int chunk_len,
-                                                             const uint32_t* __restrict__ keys, float scale,
-                                                             const float* __restrict__ slots, T* __restrict__ dweight) {
-  __shared__ float sums[EMB_JOIN_THREADS];
-  const long long chunk = blockIdx.x, begin = chunk * chunk_len, end = begin + chunk_len;  // end < n: a border
-  const uint32_t key = keys[end - 1];
-  if (key == vocab || keys[end] != key) return;
-  if (begin > 0 && keys[begin - 1] == key) return;  // it began earlier
-  // the end of its run, by bisection
-  long long lo = end, hi = n;
-  while (hi - lo > 1) {
-    const long long m = (lo + hi) >> 1;
-    if (keys[m] == key) lo = m;
-    else hi = m;
-  }
-  const long long last = lo / chunk_len;
-  const int parts = EMB_JOIN_THREADS / lanes, part = threadIdx.x / lanes;
-  for (int base = 0; base < width; base += lanes) {
-    const int c = base + threadIdx.x % lanes;
+__global__ void __launch_bounds__(EMB_THREADS) emb_join(int n, int width, int chunk_len, const uint32_t* __restrict__ keys,
+                                                        float scale, const float* __restrict__ slots,
+                                                        const uint32_t* __restrict__ runs, T* __restrict__ dweight) {
+  __shared__ float sums[EMB_THREADS];
+  const long long chunks = (n - 1LL) / chunk_len + 1;
+  const int slabs = (width + EMB_JOIN_COLS - 1) / EMB_JOIN_COLS;
+  const long long items = (long long)runs[0] * slabs;
+  for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+    const long long chunk = runs[1 + item / slabs];
+    const uint32_t key = keys[(chunk + 1) * chunk_len];
+    // the last chunk that begins inside the run: in steps that double, then by halves
+    long long last = chunk + 1, step = 1;
+    while (last + step < chunks && keys[(last + step) * chunk_len] == key) {
+      last += step;
+      step *= 2;
+    }
+    for (; step > 0; step >>= 1)
+      if (last + step < chunks && keys[(last + step) * chunk_len] == key) last += step;
+    const int c = (int)(item % slabs) * EMB_JOIN_COLS + (threadIdx.x & 63), part = threadIdx.x >> 6;
     float acc = 0.0f;
     if (c < width) {
 #pragma unroll 8
-      for (long long k = chunk + 1 + part; k <= last; k += parts) acc += slots[2 * k * width + c];
+      for (long long k = chunk + 1 + part; k <= last; k += EMB_THREADS / 64) acc += slots[2 * k * width + c];
     }
     sums[threadIdx.x] = acc;
     __syncthreads();
     if (part == 0 && c < width) {
       acc += slots[(2 * chunk + 1) * width + c];
-      for (int p = 1; p < parts; ++p) acc += sums[p * lanes + threadIdx.x];
+      for (int p = 1; p < EMB_THREADS / 64; ++p) acc += sums[p * 64 + threadIdx.x];
       dweight[(long long)key * width + c] = (T)(acc * scale);
     }
     __syncthreads();
@@ -307,21 +312,21 @@ __global__ void __launch_bounds__(EMB_THREADS) emb_few(long long tokens, int voc
   const long long lo = blockIdx.x * share, hi = lo + share < tokens ? lo + share : tokens;
   float* mine = acc + threadIdx.x * W;
   if (c < width) {
-    for (long long i = lo + team; i < hi; i += (long long)teams * EMB_AHEAD) {
-      long long id[EMB_AHEAD];
-      NsaPack<T, W> row[EMB_AHEAD];
+    for (long long i = lo + team; i < hi; i += (long long)teams * EMB_FEW_AHEAD) {
+      ID id[EMB_FEW_AHEAD];
+      NsaPack<T, W> row[EMB_FEW_AHEAD];
 #pragma unroll
-      for (int j = 0; j < EMB_AHEAD; ++j) {
+      for (int j = 0; j < EMB_FEW_AHEAD; ++j) {
         const long long at = i + (long long)j * teams < hi ? i + (long long)j * teams : i;
-        id[j] = (long long)ids[at];
+        id[j] = ids[at];
         row[j] = *reinterpret_cast<const NsaPack<T, W>*>(dy + at * width + c);
       }
 #pragma unroll
-      for (int j = 0; j < EMB_AHEAD; ++j) {
+      for (int j = 0; j < EMB_FEW_AHEAD; ++j) {
         if (i + (long long)j * teams < hi && id[j] >= 0 && id[j] < vocab && id[j] != padding) {
           float* p = mine + (int)id[j] * EMB_THREADS * W;
 #pragma unroll
-          for (int w = 0; w < W; ++w) p[w] += (float)row[j].v[w];
+          for (int w = 0; w < W; ++w) p[w] += (float)row[j].v[w];  // (LDS float atomics take three times as long)
         }
       }
     }
@@ -389,10 +394,17 @@ int emb_passes(long long vocab) {  // 8 bits each; the largest key is `vocab` it
   return (bits + 7) / 8;
 }
 
+// Sorting tiles.  A few hundred thousand tokens in tiles of 4096 would leave most compute units idle: 131072 tokens, a pass of
+// 22 us in 32 tiles.
+long long emb_tiles(long long n) {
+  const int tile = EMB_THREADS * (n < EMB_MANY ? 4 : 16);
+  return (n + tile - 1) / tile;
+}
+
 // sorted positions per team of the reduction: short chunks for few tokens (all compute units at work), longer ones for many
 // (fewer partial sums to join)
 int emb_chunk(long long n) {
-  int len = 16;
+  int len = 32;
   while (len < 256 && n / len > 16384) len *= 2;
   return len;
 }
@@ -413,15 +425,15 @@ EmbFew emb_few_plan(long long n, long long vocab, int width, int bytes) {
   f.lanes = 1;
   while (f.lanes < 64 && f.lanes < vectors) f.lanes *= 2;
   f.slabs = (vectors + f.lanes - 1) / f.lanes;
-  const long long step = (long long)(EMB_THREADS / f.lanes) * EMB_AHEAD;  // tokens of a workgroup in flight
-  const long long blocks = std::max(1LL, std::min(1024LL / f.slabs + 1, n / (4 * step)));
+  const long long step = (long long)(EMB_THREADS / f.lanes) * EMB_FEW_AHEAD;  // tokens of a workgroup in flight
+  const long long blocks = std::max(1LL, std::min(1024LL / f.slabs + 1, n / step));
   f.share = (n + blocks - 1) / blocks;
   f.blocks = (int)((n + f.share - 1) / f.share);
   return f;
 }
 
 struct EmbSpace {
-  uint32_t *keys[2], *pos[2], *counts, *totals;
+  uint32_t *keys[2], *pos[2], *counts, *totals, *runs;
   float* slots;
   size_t bytes;
 };
@@ -434,13 +446,14 @@ EmbSpace emb_space(char* p, long long n, int width) {
     at += (bytes + 255) & ~(size_t)255;
     return q;
   };
-  const long long tiles = (n + EMB_TILE - 1) / EMB_TILE, chunks = (n + emb_chunk(n) - 1) / emb_chunk(n);
+  const long long tiles = emb_tiles(n), chunks = (n + emb_chunk(n) - 1) / emb_chunk(n);
   for (int i = 0; i < 2; ++i) {
     w.keys[i] = (uint32_t*)take(n * 4);
     w.pos[i] = (uint32_t*)take(n * 4);
   }
   w.counts = (uint32_t*)take(tiles * 256 * 4);
   w.totals = (uint32_t*)take(256 * 4);
+  w.runs = (uint32_t*)take((1 + chunks) * 4);
   w.slots = (float*)take((size_t)chunks * 2 * width * 4);
   w.bytes = at;
   return w;
@@ -489,13 +502,11 @@ void emb_reduce_launch(int n, long long vocab, int width, const EmbSpace& w, int
   const int slabs = (width + lanes * V - 1) / (lanes * V);
   hipLaunchKernelGGL((emb_reduce<T, V>), dim3((unsigned)((chunks + teams - 1) / teams), slabs), dim3(EMB_THREADS), 0, s, n,
                      (uint32_t)vocab, width, lanes, len, w.keys[side], w.pos[side], (const T*)dy, scale, (T*)dweight,
-                     w.slots);
-  const long long borders = ((long long)n - 1) / len;
-  int across = 16;
-  while (across < EMB_JOIN_THREADS && across < width) across *= 2;
+                     w.slots, w.runs);
+  const long long borders = ((long long)n - 1) / len, items = borders * ((width + EMB_JOIN_COLS - 1) / EMB_JOIN_COLS);
   if (borders > 0)
-    hipLaunchKernelGGL((emb_join<T>), dim3((unsigned)borders), dim3(EMB_JOIN_THREADS), 0, s, n, (uint32_t)vocab, width, across,
-                       len, w.keys[side], scale, w.slots, (T*)dweight);
+    hipLaunchKernelGGL((emb_join<T>), dim3((unsigned)std::min(items, 2048LL)), dim3(EMB_THREADS), 0, s, n, width, len,
+                       w.keys[side], scale, w.slots, w.runs, (T*)dweight);
 }
 
 template <typename T, typename ID, int W>
@@ -509,19 +520,26 @@ void emb_few_launch(const EmbFew& f, long long n, int vocab, int width, const vo
                      f.blocks, part, scale, (T*)dweight);
 }
 
-template <typename ID>
+template <typename ID, int ITEMS>
 int emb_sort(int n, long long vocab, const ID* ids, long long padding, const EmbSpace& w, hipStream_t s) {
-  const unsigned tiles = (unsigned)(((long long)n + EMB_TILE - 1) / EMB_TILE);
+  const unsigned tiles = (unsigned)emb_tiles(n);
   const int passes = emb_passes(vocab);
   for (int p = 0; p < passes; ++p) {
     const uint32_t* keys = p == 0 ? nullptr : w.keys[p & 1];
     const uint32_t* pos = p == 0 ? nullptr : w.pos[p & 1];
-    hipLaunchKernelGGL((emb_count<ID>), dim3(tiles), dim3(EMB_THREADS), 0, s, n, ids, vocab, padding, keys, 8 * p, w.counts);
+    hipLaunchKernelGGL((emb_count<ID, ITEMS>), dim3(tiles), dim3(EMB_THREADS), 0, s, n, ids, vocab, padding, keys, 8 * p,
+                       w.counts);
     hipLaunchKernelGGL(emb_scan, dim3(256), dim3(EMB_THREADS), 0, s, (int)tiles, w.counts, w.totals);
-    hipLaunchKernelGGL((emb_scatter<ID>), dim3(tiles), dim3(EMB_THREADS), 0, s, n, ids, vocab, padding, keys, pos, 8 * p,
-                       w.counts, w.totals, w.keys[(p + 1) & 1], w.pos[(p + 1) & 1]);
+    hipLaunchKernelGGL((emb_scatter<ID, ITEMS>), dim3(tiles), dim3(EMB_THREADS), 0, s, n, ids, vocab, padding, keys, pos,
+                       8 * p, w.counts, w.totals, w.keys[(p + 1) & 1], w.pos[(p + 1) & 1]);
   }
   return passes & 1;
+}
+
+template <typename ID>
+int emb_sort(int n, long long vocab, const void* ids, long long padding, const EmbSpace& w, hipStream_t s) {
+  return n < EMB_MANY ? emb_sort<ID, 4>(n, vocab, (const ID*)ids, padding, w, s)
+                      : emb_sort<ID, 16>(n, vocab, (const ID*)ids, padding, w, s);
 }
 
 template <typename T>
@@ -541,10 +559,9 @@ void emb_backward_typed(int n, long long vocab, int width, const void* ids, int 
   }
   const long long cells = vocab * width;
   hipLaunchKernelGGL((emb_zero<T>), dim3((unsigned)std::min((cells + EMB_THREADS - 1) / EMB_THREADS, 8192LL)),
-                     dim3(EMB_THREADS), 0, s, cells, (T*)dweight);
+                     dim3(EMB_THREADS), 0, s, cells, (T*)dweight, n == 0 ? nullptr : w.runs);
   if (n == 0) return;  // (all rows are zero)
-  const int side = ids_bytes == 4 ? emb_sort<int>(n, vocab, (const int*)ids, padding, w, s)
-                                  : emb_sort<long long>(n, vocab, (const long long*)ids, padding, w, s);
+  const int side = ids_bytes == 4 ? emb_sort<int>(n, vocab, ids, padding, w, s) : emb_sort<long long>(n, vocab, ids, padding, w, s);
   const int v = emb_vector(width, sizeof(T), (uintptr_t)dy | (uintptr_t)dweight);
   if constexpr (sizeof(T) == 2) {
     if (v == 8) return emb_reduce_launch<T, 8>(n, vocab, width, w, side, dy, scale, dweight, s);

@@ -105,6 +105,26 @@ __device__ __forceinline__ GnPlace gn_place(const GnShape& s) {
   return p;
 }
 
+// This thread's positions of the chunk, GN_AHEAD at a time: ask(slot, offset) for all of them, then use(slot, offset).  The
+// offset is that of the thread's channels c at a position.
+#define GN_AHEAD 4
+template <typename ASK, typename USE>
+__device__ __forceinline__ void gn_positions(const GnShape& s, const GnPlace& p, int c, ASK ask, USE use) {
+  const long long row = (long long)s.rows * s.channels;
+  long long at = (p.n * s.length + p.l0 + p.r) * s.channels + p.slab * s.width + c;
+  long long l = p.l0 + p.r;
+  for (; l + (GN_AHEAD - 1) * s.rows < p.l1; l += GN_AHEAD * s.rows, at += GN_AHEAD * row) {
+#pragma unroll
+    for (int k = 0; k < GN_AHEAD; ++k) ask(k, at + k * row);
+#pragma unroll
+    for (int k = 0; k < GN_AHEAD; ++k) use(k, at + k * row);
+  }
+  for (; l < p.l1; l += s.rows, at += row) {
+    ask(0, at);
+    use(0, at);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
@@ -123,22 +143,21 @@ __global__ void __launch_bounds__(GN_THREADS) gn_stats(GnShape s, const T* __res
     for (int t = 0; t < s.tiles; ++t) {
       const int c = (t * s.vecs + p.j) * V;
       if (c >= s.width) break;
-      const T* px = x + (p.n * s.length + p.l0 + p.r) * s.channels + p.slab * s.width + c;
-      for (long long l = p.l0 + p.r; l < p.l1; l += s.rows, px += (long long)s.rows * s.channels) {
-        float v[V];
-        nsa_load<T, V>(px, v);
-        if (count == 0) {
+      NsaPack<T, V> px[GN_AHEAD];
+      gn_positions(s, p, c, [&](int k, long long at) { px[k] = *reinterpret_cast<const NsaPack<T, V>*>(x + at); },
+                   [&](int k, long long) {
+                     if (count == 0) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) shift[i] = v[i];
-        }
+                       for (int i = 0; i < V; ++i) shift[i] = (float)px[k].v[i];
+                     }
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float d = v[i] - shift[i];
-          sum[i] += d;
-          sq[i] = fmaf(d, d, sq[i]);
-        }
-        ++count;
-      }
+                     for (int i = 0; i < V; ++i) {
+                       const float d = (float)px[k].v[i] - shift[i];
+                       sum[i] += d;
+                       sq[i] = fmaf(d, d, sq[i]);
+                     }
+                     ++count;
+                   });
     }
   }
   const float inv = count > 0 ? 1.0f / (float)count : 0.0f;
@@ -150,51 +169,65 @@ __global__ void __launch_bounds__(GN_THREADS) gn_stats(GnShape s, const T* __res
     devs[threadIdx.x * V + i] = fmaxf(sq[i] - sum[i] * d, 0.0f);
   }
   __syncthreads();
-  // a wave per group joins the parts: rows x (channels of the group in a tile), in a fixed order
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // A team of lanes per group joins the parts - rows x (channels of the group in a tile) - in a fixed order; as many lanes
+  // as give every group of the slab a team.
   const int span = s.vecs * V;                              // channels in the parts of a row
   const int in_group = s.cpg < span ? s.cpg : span;         // of them, in one group
-  const long long rows_here = p.l1 - p.l0;
-  const float total = (float)rows_here * (float)s.cpg;
-  for (int g = wave; g < s.gps; g += GN_THREADS / 64) {
-    const int first = g * s.cpg, parts = in_group * s.rows;
+  const int parts = in_group * s.rows;
+  int team = 1;
+  while (team < 64 && team * 2 * s.gps <= GN_THREADS && team * 2 <= parts) team *= 2;
+  const int lane = threadIdx.x & (team - 1);
+  const float total = (float)(p.l1 - p.l0) * (float)s.cpg;
+  for (int g = threadIdx.x / team; g < s.gps; g += GN_THREADS / team) {
+    const int first = g * s.cpg;
     float a = 0.0f;
-    for (int e = lane; e < parts; e += 64) {
-      const int c = first + e % in_group, r = e / in_group, t = r * s.vecs + c / V;
-      a += (float)counts[t] * means[r * span + c];
+    for (int e = lane; e < parts; e += team) {
+      const int r = e / in_group, c = first + e - r * in_group;
+      a += (float)counts[r * s.vecs + c / V] * means[r * span + c];
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) a += __shfl_xor(a, o);
+    for (int o = team >> 1; o > 0; o >>= 1) a += __shfl_xor(a, o);
     const float mean = a / total;
     float m2 = 0.0f;
-    for (int e = lane; e < parts; e += 64) {
-      const int c = first + e % in_group, r = e / in_group, t = r * s.vecs + c / V;
+    for (int e = lane; e < parts; e += team) {
+      const int r = e / in_group, c = first + e - r * in_group, count_here = counts[r * s.vecs + c / V];
       const float d = means[r * span + c] - mean;
-      m2 += devs[r * span + c] + (counts[t] > 0 ? (float)counts[t] * d * d : 0.0f);
+      m2 += devs[r * span + c] + (count_here > 0 ? (float)count_here * d * d : 0.0f);
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m2 += __shfl_xor(m2, o);
+    for (int o = team >> 1; o > 0; o >>= 1) m2 += __shfl_xor(m2, o);
     if (lane == 0) part[(p.n * s.chunks + p.chunk) * s.groups + p.slab * s.gps + g] = make_float2(mean, m2);
   }
 }
 
-// the chunks of a (sample, group) joined; a thread each
+// the chunks of a (sample, group) joined in 64 bits: a wave each, lane by lane, then lane with lane
 __global__ void __launch_bounds__(GN_THREADS) gn_stats_join(GnShape s, const float2* __restrict__ part, float eps,
                                                             float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-  const long long i = (long long)blockIdx.x * GN_THREADS + threadIdx.x;
+  const long long i = (long long)blockIdx.x * (GN_THREADS / 64) + (threadIdx.x >> 6);
   if (i >= s.samples * s.groups) return;
   const long long n = i / s.groups, g = i % s.groups;
+  const int lane = threadIdx.x & 63;
   double mean = 0.0, m2 = 0.0, count = 0.0;
-  for (int k = 0; k < s.chunks; ++k) {
+  auto join = [&](double mean_b, double m2_b, double count_b) {
+    const double all = count + count_b, d = mean_b - mean;
+    if (all > 0.0) {
+      mean += d * (count_b / all);
+      m2 += m2_b + d * d * (count * count_b / all);
+      count = all;
+    }
+  };
+  for (int k = lane; k < s.chunks; k += 64) {
     const float2 q = part[(n * s.chunks + k) * s.groups + g];
     const long long l0 = k * s.chunk, rows = (l0 + s.chunk < s.length ? l0 + s.chunk : s.length) - l0;
-    const double c = (double)rows * s.cpg, d = (double)q.x - mean, all = count + c;
-    mean += d * (c / all);
-    m2 += (double)q.y + d * d * (count * c / all);
-    count = all;
+    join((double)q.x, (double)q.y, (double)rows * s.cpg);
   }
-  mean_out[i] = (float)mean;
-  rstd_out[i] = (float)(1.0 / sqrt(m2 / count + (double)eps));
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double mean_b = __shfl_down(mean, o), m2_b = __shfl_down(m2, o), count_b = __shfl_down(count, o);
+    if (lane + o < 64) join(mean_b, m2_b, count_b);  // (lane 0 ends with all of them, in order)
+  }
+  if (lane == 0) {
+    mean_out[i] = (float)mean;
+    rstd_out[i] = (float)(1.0 / sqrt(m2 / count + (double)eps));
+  }
 }
 
 template <typename T, int V, int ACT>
@@ -215,14 +248,14 @@ __global__ void __launch_bounds__(GN_THREADS) gn_apply(GnShape s, const T* __res
       w[i] = gn_param<T>(q.w, q.f32, ch, 1.0f);
       b[i] = gn_param<T>(q.b, q.f32, ch, 0.0f);
     }
-    long long at = (p.n * s.length + p.l0 + p.r) * s.channels + p.slab * s.width + c;
-    for (long long l = p.l0 + p.r; l < p.l1; l += s.rows, at += (long long)s.rows * s.channels) {
-      float v[V];
-      nsa_load<T, V>(x + at, v);
+    NsaPack<T, V> px[GN_AHEAD];
+    gn_positions(s, p, c, [&](int k, long long at) { px[k] = *reinterpret_cast<const NsaPack<T, V>*>(x + at); },
+                 [&](int k, long long at) {
+                   float v[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = gn_act<ACT>(fmaf((v[i] - mu[i]) * rs[i], w[i], b[i]));
-      nsa_store<T, V>(y + at, v);
-    }
+                   for (int i = 0; i < V; ++i) v[i] = gn_act<ACT>(fmaf(((float)px[k].v[i] - mu[i]) * rs[i], w[i], b[i]));
+                   nsa_store<T, V>(y + at, v);
+                 });
   }
 }
 
@@ -252,19 +285,21 @@ __global__ void __launch_bounds__(GN_THREADS) gn_sums(GnShape s, const T* __rest
         w[i] = gn_param<T>(q.w, q.f32, ch, 1.0f);
         b[i] = gn_param<T>(q.b, q.f32, ch, 0.0f);
       }
-      long long at = (p.n * s.length + p.l0 + p.r) * s.channels + p.slab * s.width + c;
-      for (long long l = p.l0 + p.r; l < p.l1; l += s.rows, at += (long long)s.rows * s.channels) {
-        float v[V], g[V];
-        nsa_load<T, V>(x + at, v);
-        nsa_load<T, V>(dy + at, g);
+      NsaPack<T, V> px[GN_AHEAD], pd[GN_AHEAD];
+      gn_positions(s, p, c,
+                   [&](int k, long long at) {
+                     px[k] = *reinterpret_cast<const NsaPack<T, V>*>(x + at);
+                     pd[k] = *reinterpret_cast<const NsaPack<T, V>*>(dy + at);
+                   },
+                   [&](int k, long long) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float xh = (v[i] - mu[i]) * rs[i];
-          const float dz = g[i] * gn_slope<ACT>(fmaf(xh, w[i], b[i]));
-          s1[i] += dz;
-          s2[i] = fmaf(dz, xh, s2[i]);
-        }
-      }
+                     for (int i = 0; i < V; ++i) {
+                       const float xh = ((float)px[k].v[i] - mu[i]) * rs[i];
+                       const float dz = (float)pd[k].v[i] * gn_slope<ACT>(fmaf(xh, w[i], b[i]));
+                       s1[i] += dz;
+                       s2[i] = fmaf(dz, xh, s2[i]);
+                     }
+                   });
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) red[threadIdx.x * V + i] = make_float2(s1[i], s2[i]);
@@ -285,35 +320,53 @@ __global__ void __launch_bounds__(GN_THREADS) gn_sums(GnShape s, const T* __rest
   }
 }
 
-// A wave per (sample, group): the chunks' sums joined into chunk 0's place, and the group's A and B
+// A workgroup per (sample, group): the chunks' sums joined into chunk 0's place, and the group's A and B.  `across` threads
+// (a power of two) lie along the channels, the others share the chunks out.
 template <typename T>
-__global__ void __launch_bounds__(GN_THREADS) gn_sums_join(GnShape s, float2* __restrict__ part, GnParams q,
+__global__ void __launch_bounds__(GN_THREADS) gn_sums_join(GnShape s, int across, float2* __restrict__ part, GnParams q,
                                                            float2* __restrict__ ab) {
-  const long long i = (long long)blockIdx.x * (GN_THREADS / 64) + (threadIdx.x >> 6);
-  if (i >= s.samples * s.groups) return;
-  const long long n = i / s.groups;
-  const int g = (int)(i % s.groups), lane = threadIdx.x & 63;
-  float a = 0.0f, b = 0.0f;
-  for (int c = g * s.cpg + lane; c < (g + 1) * s.cpg; c += 64) {
-    float2* first = part + n * s.chunks * s.channels + c;
-    float2 t = first[0];
-    for (int k = 1; k < s.chunks; ++k) {
-      const float2 o = first[(long long)k * s.channels];
-      t.x += o.x;
-      t.y += o.y;
+  __shared__ float2 red[GN_THREADS];
+  const long long n = blockIdx.x / s.groups;
+  const int g = (int)(blockIdx.x % s.groups), lane = threadIdx.x % across, share = threadIdx.x / across;
+  const int shares = GN_THREADS / across;
+  float2 t = make_float2(0.0f, 0.0f);  // this thread's part of A and B
+  for (int base = 0; base < s.cpg; base += across) {
+    const int c = g * s.cpg + base + lane;
+    float2 a = make_float2(0.0f, 0.0f);
+    if (base + lane < s.cpg) {
+      const float2* p = part + n * s.chunks * s.channels + c;
+#pragma unroll 4
+      for (int k = share; k < s.chunks; k += shares) {
+        const float2 o = p[(long long)k * s.channels];
+        a.x += o.x;
+        a.y += o.y;
+      }
     }
-    first[0] = t;
-    const float w = gn_param<T>(q.w, q.f32, c, 1.0f);
-    a = fmaf(w, t.x, a);
-    b = fmaf(w, t.y, b);
+    red[threadIdx.x] = a;
+    __syncthreads();
+    if (share == 0 && base + lane < s.cpg) {
+      for (int k = 1; k < shares; ++k) {
+        a.x += red[k * across + lane].x;
+        a.y += red[k * across + lane].y;
+      }
+      part[n * s.chunks * s.channels + c] = a;
+      const float w = gn_param<T>(q.w, q.f32, c, 1.0f);
+      t.x = fmaf(w, a.x, t.x);
+      t.y = fmaf(w, a.y, t.y);
+    }
+    __syncthreads();
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    a += __shfl_xor(a, o);
-    b += __shfl_xor(b, o);
+  red[threadIdx.x] = t;
+  __syncthreads();
+  for (int half = across >> 1; half > 0; half >>= 1) {
+    if (threadIdx.x < half) {
+      red[threadIdx.x].x += red[threadIdx.x + half].x;
+      red[threadIdx.x].y += red[threadIdx.x + half].y;
+    }
+    __syncthreads();
   }
   const float m = (float)s.length * (float)s.cpg;
-  if (lane == 0) ab[i] = make_float2(a / m, b / m);
+  if (threadIdx.x == 0) ab[blockIdx.x] = make_float2(red[0].x / m, red[0].y / m);
 }
 
 template <typename T, int V, int ACT>
@@ -337,19 +390,22 @@ __global__ void __launch_bounds__(GN_THREADS) gn_dx(GnShape s, const T* __restri
       w[i] = gn_param<T>(q.w, q.f32, ch, 1.0f);
       b[i] = gn_param<T>(q.b, q.f32, ch, 0.0f);
     }
-    long long at = (p.n * s.length + p.l0 + p.r) * s.channels + p.slab * s.width + c;
-    for (long long l = p.l0 + p.r; l < p.l1; l += s.rows, at += (long long)s.rows * s.channels) {
-      float v[V], g[V];
-      nsa_load<T, V>(x + at, v);
-      nsa_load<T, V>(dy + at, g);
+    NsaPack<T, V> px[GN_AHEAD], pd[GN_AHEAD];
+    gn_positions(s, p, c,
+                 [&](int k, long long at) {
+                   px[k] = *reinterpret_cast<const NsaPack<T, V>*>(x + at);
+                   pd[k] = *reinterpret_cast<const NsaPack<T, V>*>(dy + at);
+                 },
+                 [&](int k, long long at) {
+                   float v[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float xh = (v[i] - mu[i]) * rs[i];
-        const float dz = g[i] * gn_slope<ACT>(fmaf(xh, w[i], b[i]));
-        v[i] = rs[i] * (w[i] * dz - ga[i] - xh * gb[i]);
-      }
-      nsa_store<T, V>(dx + at, v);
-    }
+                   for (int i = 0; i < V; ++i) {
+                     const float xh = ((float)px[k].v[i] - mu[i]) * rs[i];
+                     const float dz = (float)pd[k].v[i] * gn_slope<ACT>(fmaf(xh, w[i], b[i]));
+                     v[i] = rs[i] * (w[i] * dz - ga[i] - xh * gb[i]);
+                   }
+                   nsa_store<T, V>(dx + at, v);
+                 });
   }
 }
 
@@ -623,12 +679,138 @@ __global__ void __launch_bounds__(THREADS) gn_tile_backward(GnTile q, const T* _
 }
 
 // ---------------------------------------------------------------------------
+// rows of a power of two of channels: no LDS, no division
+// ---------------------------------------------------------------------------
+
+// length 1, channels and channels per group powers of two: a group is a power of two of neighbouring lanes, which add by
+// shuffles; a thread's accesses all lie in the same V channels, whose parameters and column sums it keeps in registers.
+struct GnRows {
+  long long vectors;  // samples * channels / V
+  int vecs;           // accesses of a row (a power of two, at most GN_THREADS)
+  int span;           // lanes of a group (a power of two, at most 64)
+  int channels, groups;
+};
+#define GN_ROW_STEPS 4  // accesses of a thread in flight
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(GN_THREADS) gn_rows_forward(GnRows q, const T* __restrict__ x, GnParams par, float eps,
+                                                              float* __restrict__ mean, float* __restrict__ rstd,
+                                                              T* __restrict__ y) {
+  const int c = (threadIdx.x & (q.vecs - 1)) * V;
+  float w[V], b[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    w[i] = gn_param<T>(par.w, par.f32, c + i, 1.0f);
+    b[i] = gn_param<T>(par.b, par.f32, c + i, 0.0f);
+  }
+  const float inv = 1.0f / (float)(q.span * V);
+  const long long base = (long long)blockIdx.x * GN_THREADS * GN_ROW_STEPS + threadIdx.x;
+  float v[GN_ROW_STEPS][V];
+#pragma unroll
+  for (int k = 0; k < GN_ROW_STEPS; ++k)
+    if (base + k * GN_THREADS < q.vectors) nsa_load<T, V>(x + (base + k * GN_THREADS) * V, v[k]);
+#pragma unroll
+  for (int k = 0; k < GN_ROW_STEPS; ++k) {
+    const long long e = base + k * GN_THREADS;
+    if (e >= q.vectors) break;  // (whole rows: the lanes of a group leave together)
+    const float shift = __shfl(v[k][0], (threadIdx.x & 63) & ~(q.span - 1));
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) s += v[k][i] - shift;
+    for (int o = q.span >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    const float mu = fmaf(s, inv, shift);
+    float d2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) d2 = fmaf(v[k][i] - mu, v[k][i] - mu, d2);
+    for (int o = q.span >> 1; o > 0; o >>= 1) d2 += __shfl_xor(d2, o);
+    const float rs = 1.0f / sqrtf(fmaf(d2, inv, eps));
+    if ((threadIdx.x & (q.span - 1)) == 0) {
+      mean[e / q.span] = mu;
+      rstd[e / q.span] = rs;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[k][i] = gn_act<ACT>(fmaf((v[k][i] - mu) * rs, w[i], b[i]));
+    nsa_store<T, V>(y + e * V, v[k]);
+  }
+}
+
+// part[block][channels]: the column sums of this workgroup's rows
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(GN_THREADS) gn_rows_backward(GnRows q, const T* __restrict__ x, const T* __restrict__ dy,
+                                                               GnParams par, const float* __restrict__ mean,
+                                                               const float* __restrict__ rstd, T* __restrict__ dx,
+                                                               float2* __restrict__ part) {
+  const int c = (threadIdx.x & (q.vecs - 1)) * V;
+  float w[V], b[V], s1[V], s2[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    w[i] = gn_param<T>(par.w, par.f32, c + i, 1.0f);
+    b[i] = gn_param<T>(par.b, par.f32, c + i, 0.0f);
+    s1[i] = s2[i] = 0.0f;
+  }
+  const float inv = 1.0f / (float)(q.span * V);
+  const long long step = (long long)gridDim.x * GN_THREADS * GN_ROW_STEPS;
+  for (long long base = (long long)blockIdx.x * GN_THREADS * GN_ROW_STEPS + threadIdx.x; base < q.vectors; base += step) {
+    NsaPack<T, V> px[GN_ROW_STEPS], pd[GN_ROW_STEPS];
+    float mu[GN_ROW_STEPS], rs[GN_ROW_STEPS];
+#pragma unroll
+    for (int k = 0; k < GN_ROW_STEPS; ++k) {
+      const long long e = base + k * GN_THREADS;
+      if (e < q.vectors) {
+        px[k] = *reinterpret_cast<const NsaPack<T, V>*>(x + e * V);
+        pd[k] = *reinterpret_cast<const NsaPack<T, V>*>(dy + e * V);
+        mu[k] = mean[e / q.span];
+        rs[k] = rstd[e / q.span];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < GN_ROW_STEPS; ++k) {
+      const long long e = base + k * GN_THREADS;
+      if (e >= q.vectors) break;
+      float xh[V], dz[V], a = 0.0f, ax = 0.0f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        xh[i] = ((float)px[k].v[i] - mu[k]) * rs[k];
+        dz[i] = (float)pd[k].v[i] * gn_slope<ACT>(fmaf(xh[i], w[i], b[i]));
+        s1[i] += dz[i];
+        s2[i] = fmaf(dz[i], xh[i], s2[i]);
+        dz[i] *= w[i];
+        a += dz[i];
+        ax = fmaf(dz[i], xh[i], ax);
+      }
+      for (int o = q.span >> 1; o > 0; o >>= 1) {
+        a += __shfl_xor(a, o);
+        ax += __shfl_xor(ax, o);
+      }
+      a *= inv;
+      ax *= inv;
+#pragma unroll
+      for (int i = 0; i < V; ++i) dz[i] = rs[k] * (dz[i] - a - xh[i] * ax);
+      if (dx != nullptr) nsa_store<T, V>(dx + e * V, dz);
+    }
+  }
+  if (part == nullptr) return;
+  __shared__ float2 red[GN_THREADS * V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) red[threadIdx.x * V + i] = make_float2(s1[i], s2[i]);
+  __syncthreads();
+  for (int ch = threadIdx.x; ch < q.channels; ch += GN_THREADS) {
+    float2 t = red[ch];
+    for (int r = q.channels; r < GN_THREADS * V; r += q.channels) {
+      t.x += red[r + ch].x;
+      t.y += red[r + ch].y;
+    }
+    part[(long long)blockIdx.x * q.channels + ch] = t;
+  }
+}
+
+// ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 namespace {
 
 // workgroups wanted of a launch: a few for each of the 256 compute units, so that no unit waits for a long one
-const long long GN_GROUPS_WANTED = 2048;
+const long long GN_GROUPS_WANTED = 1024;
 // positions of a chunk at least, per row of threads: below it a workgroup's start costs more than its work
 const long long GN_CHUNK_ROWS = 8;
 
@@ -641,6 +823,8 @@ GnShape gn_shape(long long samples, long long length, int channels, int groups, 
   s.cpg = channels / groups;
   v = 16 / bytes;
   while (v > 1 && (channels % v != 0 || addresses % (uintptr_t)(v * bytes) != 0)) v >>= 1;
+  if (length == 1 && (channels & (channels - 1)) == 0 && s.cpg >= 2)  // (gn_rows: no access over two groups)
+    while (v > s.cpg) v >>= 1;
   for (;; v >>= 1) {  // the widest access with which slabs of whole groups begin at a multiple of it
     const int most = GN_THREADS * v;
     s.gps = groups;
@@ -665,7 +849,7 @@ GnShape gn_shape(long long samples, long long length, int channels, int groups, 
 }
 
 const size_t GN_LDS = 152 * 1024;  // of a workgroup's 160 KB
-const int GN_TILE_BLOCKS = 1024;  // workgroups of the backward tiles: one record of column sums each
+const int GN_TILE_BLOCKS = 1024;  // workgroups of the one-pass backward kernels: one record of column sums each
 
 bool gn_tile(long long samples, long long length, int channels, int groups, int v, int most, GnTile& q) {
   if (length * channels > most) return false;
@@ -690,6 +874,17 @@ bool gn_tile(long long samples, long long length, int channels, int groups, int 
   return true;
 }
 
+bool gn_rows(const GnShape& s, int v, GnRows& q) {
+  if (s.length != 1 || (s.channels & (s.channels - 1)) != 0 || s.cpg < v) return false;  // (groups divides a power of two)
+  q.vecs = s.channels / v;
+  q.span = s.cpg / v;
+  if (q.vecs > GN_THREADS || q.span > 64) return false;
+  q.vectors = s.samples * q.vecs;
+  q.channels = s.channels;
+  q.groups = s.groups;
+  return true;
+}
+
 // An upper bound that does not ask for the addresses: chunks do not grow with a narrower access by more than the rows do
 size_t gn_workspace(long long samples, long long length, int channels, int groups, int bytes, bool backward) {
   size_t most = 0;
@@ -699,7 +894,7 @@ size_t gn_workspace(long long samples, long long length, int channels, int group
     const size_t parts = (size_t)s.samples * s.chunks * (backward ? s.channels : s.groups) * sizeof(float2);
     most = std::max(most, parts);
   }
-  if (backward && length * channels <= 256 * GN_EACH)  // the tiles' records
+  if (backward && length * channels <= 256 * GN_EACH)  // the one-pass kernels' records
     most = std::max(most, (size_t)std::min(samples, (long long)GN_TILE_BLOCKS) * channels * sizeof(float2));
   return most + (backward ? (size_t)samples * groups * sizeof(float2) : 0) + 256;
 }
@@ -746,6 +941,13 @@ int gn_done(const char* what) {
 template <typename T, int V>
 void gn_forward(const GnShape& s, const void* x, GnParams q, float eps, int act, void* y, float* mean, float* rstd,
                 float2* part, hipStream_t st) {
+  GnRows rows;
+  if (gn_rows(s, V, rows)) {
+    const long long per = GN_THREADS * GN_ROW_STEPS;
+    GN_ACTS(act, gn_rows_forward, T, V, dim3((unsigned)((rows.vectors + per - 1) / per)), dim3(GN_THREADS), 0, st, rows,
+            (const T*)x, q, eps, mean, rstd, (T*)y)
+    return;
+  }
   GnTile q_;
   for (int threads = 256; threads <= 1024; threads *= 4) {
     if (!gn_tile(s.samples, s.length, s.channels, s.groups, V, threads * GN_EACH, q_)) continue;
@@ -762,7 +964,7 @@ void gn_forward(const GnShape& s, const void* x, GnParams q, float eps, int act,
   const dim3 grid((unsigned)(s.samples * s.slabs * s.chunks)), block(GN_THREADS);
   hipLaunchKernelGGL((gn_stats<T, V>), grid, block, 0, st, s, (const T*)x, part);
   const long long pairs = s.samples * s.groups;
-  hipLaunchKernelGGL(gn_stats_join, dim3((unsigned)((pairs + GN_THREADS - 1) / GN_THREADS)), block, 0, st, s, part, eps, mean,
+  hipLaunchKernelGGL(gn_stats_join, dim3((unsigned)((pairs + GN_THREADS / 64 - 1) / (GN_THREADS / 64))), block, 0, st, s, part, eps, mean,
                      rstd);
   GN_ACTS(act, gn_apply, T, V, grid, block, 0, st, s, (const T*)x, q, mean, rstd, (T*)y)
 }
@@ -770,34 +972,41 @@ void gn_forward(const GnShape& s, const void* x, GnParams q, float eps, int act,
 template <typename T, int V>
 void gn_backward(const GnShape& s, const void* x, const void* dy, GnParams q, int act, const float* mean, const float* rstd,
                  void* dx, void* dw, void* db, float2* part, float2* ab, hipStream_t st) {
+  const bool sums = dw != nullptr || db != nullptr;
+  auto params = [&](long long count, long long stride) {
+    if (sums)
+      hipLaunchKernelGGL((gn_param_grads<T>), dim3((unsigned)((s.channels + GN_PARAM_CH - 1) / GN_PARAM_CH)),
+                         dim3(GN_PARAM_THREADS), 0, st, s.channels, count, stride, part, q.f32, dw, db);
+  };
+  GnRows rows;
+  if (gn_rows(s, V, rows)) {
+    const long long per = GN_THREADS * GN_ROW_STEPS;
+    const long long blocks = std::min((rows.vectors + per - 1) / per, (long long)GN_TILE_BLOCKS);
+    GN_ACTS(act, gn_rows_backward, T, V, dim3((unsigned)blocks), dim3(GN_THREADS), 0, st, rows, (const T*)x, (const T*)dy, q,
+            mean, rstd, (T*)dx, sums ? part : nullptr)
+    return params(blocks, s.channels);
+  }
   GnTile q_;
   if (gn_tile(s.samples, s.length, s.channels, s.groups, V, 256 * GN_EACH, q_)) {
     const size_t lds = (size_t)256 * GN_EACH * 8 + (size_t)q_.per * q_.groups * sizeof(float2) +
                        (size_t)(s.channels + 1) / 2 * 8 + (size_t)std::max(256, s.channels) * sizeof(float2);
     if (lds <= GN_LDS) {
-      const bool sums = dw != nullptr || db != nullptr;
       const int blocks = (int)std::min((s.samples + q_.per - 1) / q_.per, (long long)GN_TILE_BLOCKS);
-      GN_TILE_ACTS(act, gn_tile_backward, T, V, 256, lds, dim3(blocks), dim3(256), lds, st, q_, (const T*)x, (const T*)dy, q, mean,
-                   rstd, (T*)dx, sums ? part : nullptr)
-      if (sums)
-        hipLaunchKernelGGL((gn_param_grads<T>), dim3((unsigned)((s.channels + GN_PARAM_CH - 1) / GN_PARAM_CH)),
-                           dim3(GN_PARAM_THREADS), 0, st, s.channels, (long long)blocks, (long long)s.channels, part, q.f32,
-                           dw, db);
-      return;
+      GN_TILE_ACTS(act, gn_tile_backward, T, V, 256, lds, dim3(blocks), dim3(256), lds, st, q_, (const T*)x, (const T*)dy, q,
+                   mean, rstd, (T*)dx, sums ? part : nullptr)
+      return params(blocks, s.channels);
     }
   }
   const dim3 grid((unsigned)(s.samples * s.slabs * s.chunks)), block(GN_THREADS);
   GN_ACTS(act, gn_sums, T, V, grid, block, 0, st, s, (const T*)x, (const T*)dy, q, mean, rstd, part)
   const long long pairs = s.samples * s.groups;
-  hipLaunchKernelGGL((gn_sums_join<T>), dim3((unsigned)((pairs + GN_THREADS / 64 - 1) / (GN_THREADS / 64))), block, 0, st, s,
-                     part, q, ab);
+  int across = 1;
+  while (across < GN_THREADS && across < s.cpg) across *= 2;
+  hipLaunchKernelGGL((gn_sums_join<T>), dim3((unsigned)pairs), block, 0, st, s, across, part, q, ab);
   if (dx != nullptr) {
     GN_ACTS(act, gn_dx, T, V, grid, block, 0, st, s, (const T*)x, (const T*)dy, q, mean, rstd, ab, (T*)dx)
   }
-  if (dw != nullptr || db != nullptr)
-    hipLaunchKernelGGL((gn_param_grads<T>), dim3((unsigned)((s.channels + GN_PARAM_CH - 1) / GN_PARAM_CH)),
-                       dim3(GN_PARAM_THREADS), 0, st, s.channels, s.samples, (long long)s.chunks * s.channels, part, q.f32, dw,
-                       db);
+  params(s.samples, (long long)s.chunks * s.channels);
 }
 
 // one call per element type and access width

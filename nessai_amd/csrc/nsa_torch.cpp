@@ -1,0 +1,337 @@
+// torch operators over the C entry points of nsa_grad_norm.hip, nsa_group_norm.hip and nsa_embedding.hip
+// (torch.ops.nessai_amd.*; nessai_amd/ops_context.py documents them).  In C++ because their calls are short: a minibatch's
+// group norm runs for 5 us on the device and took 130 us, forward and backward, with the checks, allocations and the
+// autograd node in Python; clipping 300 gradients spent 220 us reading their attributes.
+//
+// Nothing here computes: arguments are checked, results and workspaces allocated, and one entry point called on the current
+// stream of the tensors' device.  The entry points' addresses come from the loaded libnessai_amd.so (nessai_amd/lib.py).
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include <cmath>
+#include <optional>
+#include <vector>
+
+#include "../../include/nessai_amd.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct EntryPoints {
+  decltype(&nsa_last_error) last_error = nullptr;
+  decltype(&nsa_grad_norm_workspace) grad_norm_workspace;
+  decltype(&nsa_grad_norm) grad_norm;
+  decltype(&nsa_grad_clip) grad_clip;
+  decltype(&nsa_group_norm_workspace) group_norm_workspace;
+  decltype(&nsa_group_norm_forward) group_norm_forward;
+  decltype(&nsa_group_norm_backward) group_norm_backward;
+  decltype(&nsa_embedding_forward) embedding_forward;
+  decltype(&nsa_embedding_workspace) embedding_workspace;
+  decltype(&nsa_embedding_backward) embedding_backward;
+};
+EntryPoints g_entry;
+
+void bind_library(at::IntArrayRef a) {  // in the order of the struct
+  TORCH_CHECK(a.size() == sizeof(EntryPoints) / sizeof(void*), "nessai_amd: wrong number of entry points");
+  for (size_t i = 0; i < a.size(); ++i) reinterpret_cast<void**>(&g_entry)[i] = reinterpret_cast<void*>(a[i]);
+}
+
+void check(int rc, const char* what) {
+  TORCH_CHECK(rc == NSA_OK, what, " failed (code ", rc, "): ", g_entry.last_error());
+}
+
+void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+int dtype_code(const Tensor& t, const char* what) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return NSA_DT_F32;
+    case at::kBFloat16: return NSA_DT_BF16;
+    case at::kHalf: return NSA_DT_F16;
+    default:
+      TORCH_CHECK_TYPE(false, what, " must be float32, bfloat16 or float16 (got ", t.scalar_type(),
+                       "): there is no kernel for other types, and nothing is cast down silently");
+  }
+}
+
+void on_device(const Tensor& t, const char* what) {
+  TORCH_CHECK(t.is_cuda(), what, ": nessai_amd operators take tensors on a ROCm device (got ", t.device(),
+              "); there is no CPU fallback");
+}
+
+Tensor workspace(const Tensor& like, size_t bytes) {
+  return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+}
+
+const void* data(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+void* mutable_data(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+
+bool wants_grad(std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : tensors)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+void once(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, " is differentiable once: its backward pass records no graph (create_graph)");
+}
+
+// -- group norm with an activation ------------------------------------------------------------------------------------
+
+struct Rows {  // of a contiguous channels-last tensor
+  int64_t samples, length, channels;
+  explicit Rows(const Tensor& x) : samples(x.size(0)), length(1), channels(x.size(-1)) {
+    for (int64_t d = 1; d + 1 < x.dim(); ++d) length *= x.size(d);
+  }
+};
+
+int param_dtype(const Tensor& weight, const Tensor& bias) {
+  const Tensor& p = weight.defined() ? weight : bias;
+  return p.defined() ? dtype_code(p, "group_norm_act: weight") : NSA_DT_F32;
+}
+
+Tensor group_norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups, double eps,
+                          int64_t activation, Tensor& stats) {
+  const Rows r(x);
+  Tensor y = at::empty(x.sizes(), x.options());
+  stats = at::empty({2, r.samples, groups}, x.options().dtype(at::kFloat));
+  if (x.numel() == 0) return y;
+  const c10::DeviceGuard guard(x.device());
+  const int code = dtype_code(x, "group_norm_act: x");
+  const size_t size = g_entry.group_norm_workspace(r.samples, r.length, r.channels, groups, code, 0);
+  const Tensor ws = workspace(x, size);
+  float* mean = (float*)stats.mutable_data_ptr();
+  check(g_entry.group_norm_forward(r.samples, r.length, r.channels, groups, code, data(x), param_dtype(weight, bias),
+                                   data(weight), data(bias), (float)eps, activation, y.mutable_data_ptr(), mean,
+                                   mean + r.samples * groups, ws.mutable_data_ptr(), size, stream_of(x)),
+        "nsa_group_norm_forward");
+  return y;
+}
+
+struct GroupNormAct : public torch::autograd::Function<GroupNormAct> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight_,
+                        const std::optional<Tensor>& bias_, int64_t groups, double eps, int64_t activation) {
+    const Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
+    Tensor stats;
+    Tensor y = group_norm_forward(x, weight, bias, groups, eps, activation, stats);
+    ctx->save_for_backward({x, weight, bias, stats});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["activation"] = activation;
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("group_norm_act");
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[3];
+    const int64_t groups = ctx->saved_data["groups"].toInt(), activation = ctx->saved_data["activation"].toInt();
+    const Rows r(x);
+    const c10::DeviceGuard guard(x.device());
+    const Tensor dy = grads[0].contiguous();
+    Tensor dx, dw, db;
+    size_t edge = 0;  // of the tensors that were given, in order
+    if (ctx->needs_input_grad(edge++)) dx = at::empty(x.sizes(), x.options());
+    if (weight.defined() && ctx->needs_input_grad(edge++)) dw = at::empty(weight.sizes(), weight.options());
+    if (bias.defined() && ctx->needs_input_grad(edge++)) db = at::empty(bias.sizes(), bias.options());
+    const int code = dtype_code(x, "group_norm_act: x");
+    const size_t size = g_entry.group_norm_workspace(r.samples, r.length, r.channels, groups, code, 1);
+    const Tensor ws = workspace(x, size);
+    const float* mean = (const float*)stats.const_data_ptr();
+    check(g_entry.group_norm_backward(r.samples, r.length, r.channels, groups, code, data(x), data(dy),
+                                      param_dtype(weight, bias), data(weight), data(bias), activation, mean,
+                                      mean + r.samples * groups, mutable_data(dx), mutable_data(dw), mutable_data(db),
+                                      ws.mutable_data_ptr(), size, stream_of(x)),
+          "nsa_group_norm_backward");
+    return {dx, dw, db, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor group_norm_act(const Tensor& x_, int64_t groups, const std::optional<Tensor>& weight_,
+                      const std::optional<Tensor>& bias_, double eps, int64_t activation) {
+  TORCH_CHECK_VALUE(x_.dim() >= 2, "expected a tensor of shape (N, ..., C), got ", x_.sizes());
+  dtype_code(x_, "group_norm_act: x");
+  const int64_t channels = x_.size(-1);
+  TORCH_CHECK_VALUE(groups >= 1 && channels >= 1 && channels % groups == 0 && channels < (1LL << 31), channels,
+                    " channels cannot be divided into ", groups, " groups");
+  TORCH_CHECK_VALUE(eps >= 0.0, "eps must not be negative (got ", eps, ")");
+  Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
+  const char* names[] = {"weight", "bias"};
+  Tensor* params[] = {&weight, &bias};
+  for (int i = 0; i < 2; ++i) {
+    Tensor& p = *params[i];
+    if (!p.defined()) continue;
+    TORCH_CHECK_VALUE(p.dim() == 1 && p.size(0) == channels, "expected a ", names[i], " of shape (", channels, ",), got ", p.sizes());
+    TORCH_CHECK_TYPE(p.scalar_type() == at::kFloat || p.scalar_type() == x_.scalar_type(), "group_norm_act: ", names[i],
+                     " must be float32 or of x's type ", x_.scalar_type(), " (got ", p.scalar_type(), ")");
+    TORCH_CHECK_VALUE(p.device() == x_.device(), "group_norm_act: ", names[i], " is on ", p.device(), ", x on ", x_.device());
+    p = p.contiguous();
+  }
+  TORCH_CHECK_TYPE(!weight.defined() || !bias.defined() || weight.scalar_type() == bias.scalar_type(),
+                   "group_norm_act: weight and bias must have one type");
+  on_device(x_, "group_norm_act");
+  const Tensor x = x_.contiguous();
+  if (wants_grad({&x, &weight, &bias})) {
+    auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+    return GroupNormAct::apply(x, given(weight), given(bias), groups, eps, activation);
+  }
+  Tensor stats;
+  return group_norm_forward(x, weight, bias, groups, eps, activation, stats);
+}
+
+// -- embedding --------------------------------------------------------------------------------------------------------
+
+Tensor embedding_forward(const Tensor& ids, const Tensor& weight, double scale) {
+  std::vector<int64_t> shape = ids.sizes().vec();
+  shape.push_back(weight.size(1));
+  Tensor out = at::empty(shape, weight.options());
+  if (out.numel() == 0) return out;
+  const c10::DeviceGuard guard(weight.device());
+  check(g_entry.embedding_forward(ids.numel(), weight.size(0), weight.size(1), dtype_code(weight, "embedding: weight"),
+                                  data(ids), (int)ids.element_size(), data(weight), (float)scale, out.mutable_data_ptr(),
+                                  stream_of(weight)),
+        "nsa_embedding_forward");
+  return out;
+}
+
+struct Embedding : public torch::autograd::Function<Embedding> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& ids, double scale, int64_t padding) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["vocab"] = weight.size(0);
+    ctx->saved_data["width"] = weight.size(1);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    return embedding_forward(ids, weight, scale);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("embedding");
+    const Tensor ids = ctx->get_saved_variables()[0], dy = grads[0].contiguous();
+    const int64_t vocab = ctx->saved_data["vocab"].toInt(), width = ctx->saved_data["width"].toInt();
+    const c10::DeviceGuard guard(dy.device());
+    Tensor dweight = at::empty({vocab, width}, dy.options());
+    const int code = dtype_code(dy, "embedding: weight");
+    const size_t size = g_entry.embedding_workspace(ids.numel(), vocab, width, code);
+    const Tensor ws = workspace(dy, size);
+    check(g_entry.embedding_backward(ids.numel(), vocab, width, code, data(ids), (int)ids.element_size(), data(dy),
+                                     (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(),
+                                     dweight.mutable_data_ptr(), ws.mutable_data_ptr(), size, stream_of(dy)),
+          "nsa_embedding_backward");
+    return {dweight, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor embedding(const Tensor& ids_, const Tensor& weight_, double scale, std::optional<int64_t> padding_idx) {
+  TORCH_CHECK_TYPE(ids_.scalar_type() == at::kInt || ids_.scalar_type() == at::kLong,
+                   "embedding: indices must be int32 or int64 (got ", ids_.scalar_type(), ")");
+  TORCH_CHECK_VALUE(weight_.dim() == 2 && weight_.size(0) >= 1 && weight_.size(1) >= 1,
+                    "embedding: expected a table of shape (V, D), got ", weight_.sizes());
+  dtype_code(weight_, "embedding: weight");
+  const int64_t vocab = weight_.size(0), most = (1LL << 31) - 1;
+  TORCH_CHECK_VALUE(vocab <= most && weight_.size(1) <= most && ids_.numel() <= most,
+                    "embedding: at most 2**31 - 1 rows, columns and indices");
+  int64_t padding = -1;
+  if (padding_idx.has_value()) {
+    TORCH_CHECK_VALUE(-vocab <= *padding_idx && *padding_idx < vocab, "embedding: padding_idx ", *padding_idx,
+                      " is outside a table of ", vocab, " rows");
+    padding = *padding_idx < 0 ? *padding_idx + vocab : *padding_idx;
+  }
+  TORCH_CHECK_VALUE(ids_.device() == weight_.device(), "embedding: indices are on ", ids_.device(), ", weight on ", weight_.device());
+  on_device(weight_, "embedding");
+  const Tensor ids = ids_.contiguous(), weight = weight_.contiguous();
+  return wants_grad({&weight}) ? Embedding::apply(weight, ids, scale, padding) : embedding_forward(ids, weight, scale);
+}
+
+// -- the norm over many gradients, and the clip -----------------------------------------------------------------------
+
+void check_gradients(const std::vector<Tensor>& tensors, const char* what) {
+  for (const Tensor& t : tensors) {
+    TORCH_CHECK_TYPE(t.layout() == at::kStrided, what, ": gradients must be dense (got ", t.layout(), ")");
+    dtype_code(t, what);
+    TORCH_CHECK_VALUE(t.device() == tensors[0].device(), what, ": gradients on several devices: ", tensors[0].device(), ", ", t.device());
+  }
+  on_device(tensors[0], what);
+}
+
+// clip: by max_norm; otherwise the norm alone.  Every tensor fills one stretch of memory.
+Tensor norm_call(const std::vector<Tensor>& tensors, int64_t kind, bool clip, double max_norm) {
+  const c10::DeviceGuard guard(tensors[0].device());
+  const int count = (int)tensors.size();
+  std::vector<void*> places(count);
+  std::vector<long long> sizes(count);
+  std::vector<int> codes(count);
+  for (int i = 0; i < count; ++i) {
+    places[i] = const_cast<void*>(tensors[i].const_data_ptr());
+    sizes[i] = tensors[i].numel();
+    codes[i] = dtype_code(tensors[i], "gradients");
+  }
+  Tensor out = at::empty({}, tensors[0].options().dtype(at::kFloat));
+  const size_t size = g_entry.grad_norm_workspace(count);
+  const Tensor ws = workspace(out, size);
+  if (clip)
+    check(g_entry.grad_clip(count, places.data(), sizes.data(), codes.data(), kind, (float)max_norm, ws.mutable_data_ptr(),
+                            size, (float*)out.mutable_data_ptr(), stream_of(out)),
+          "nsa_grad_clip");
+  else
+    check(g_entry.grad_norm(count, places.data(), sizes.data(), codes.data(), kind, ws.mutable_data_ptr(), size,
+                            (float*)out.mutable_data_ptr(), stream_of(out)),
+          "nsa_grad_norm");
+  return out;
+}
+
+Tensor grad_norm(at::TensorList tensors, int64_t kind) {
+  if (tensors.empty()) return at::zeros({}, at::kFloat);
+  const at::NoGradGuard no_grad;
+  std::vector<Tensor> grads = tensors.vec();
+  check_gradients(grads, "grad_norm: gradients");
+  for (Tensor& g : grads)
+    if (!g.is_non_overlapping_and_dense()) g = g.contiguous();
+  return norm_call(grads, kind, false, 0.0);
+}
+
+Tensor clip_grad_norm(at::TensorList parameters, int64_t kind, double max_norm, bool error_if_nonfinite) {
+  TORCH_CHECK_VALUE(max_norm >= 0.0, "max_norm must not be negative or NaN (got ", max_norm, ")");
+  const at::NoGradGuard no_grad;
+  std::vector<Tensor> grads;
+  grads.reserve(parameters.size());
+  for (const Tensor& p : parameters)
+    if (p.grad().defined()) grads.push_back(p.grad());
+  if (grads.empty()) return at::zeros({}, at::kFloat);
+  check_gradients(grads, "clip_grad_norm_: gradients");
+  // a gradient with gaps between its elements is clipped in a copy; one whose elements share memory cannot be
+  std::vector<Tensor> dense = grads;
+  for (Tensor& g : dense) {
+    if (g.is_non_overlapping_and_dense()) continue;
+    for (int64_t d = 0; d < g.dim(); ++d)
+      TORCH_CHECK_VALUE(g.stride(d) != 0 || g.size(d) <= 1,
+                        "clip_grad_norm_: a gradient's elements overlap in memory (an expanded tensor); clone it");
+    g = g.contiguous();
+  }
+  if (error_if_nonfinite)
+    TORCH_CHECK(std::isfinite(norm_call(dense, kind, false, 0.0).item<float>()),
+                "The total norm of the gradients from `parameters` is non-finite, so it cannot be clipped");
+  const Tensor norm = norm_call(dense, kind, true, max_norm);
+  for (size_t i = 0; i < grads.size(); ++i) {
+    if (!dense[i].is_same(grads[i])) grads[i].copy_(dense[i]);
+    // the kernels wrote behind torch's back: graphs that saved a gradient must see that it changed
+    else if (!grads[i].is_inference()) grads[i].unsafeGetTensorImpl()->bump_version();
+  }
+  return norm;
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(nessai_amd, m) {
+  m.def("_bind_library(int[] addresses) -> ()", &bind_library);
+  m.def("group_norm_act(Tensor x, int num_groups, Tensor? weight, Tensor? bias, float eps, int activation) -> Tensor",
+        &group_norm_act);
+  m.def("embedding(Tensor indices, Tensor weight, float scale, int? padding_idx) -> Tensor", &embedding);
+  m.def("grad_norm(Tensor[] tensors, int kind) -> Tensor", &grad_norm);
+  m.def("clip_grad_norm_(Tensor[] parameters, int kind, float max_norm, bool error_if_nonfinite) -> Tensor",
+        &clip_grad_norm);
+}

@@ -235,6 +235,38 @@ def load():
     return lib
 
 
+_TORCH_LOADED = False
+
+#: entry points that the torch operators call, in the order of ``EntryPoints`` (csrc/nsa_torch.cpp)
+_TORCH_ENTRY_POINTS = (
+    "nsa_last_error", "nsa_grad_norm_workspace", "nsa_grad_norm", "nsa_grad_clip", "nsa_group_norm_workspace",
+    "nsa_group_norm_forward", "nsa_group_norm_backward", "nsa_embedding_forward", "nsa_embedding_workspace",
+    "nsa_embedding_backward",
+)
+
+
+def load_torch():
+    """Load the torch operators (``libnessai_amd_torch.so``, next to the package's library, once) and hand them the entry
+    points of the library that ``load`` returns."""
+    global _TORCH_LOADED
+    if _TORCH_LOADED:
+        return
+    import torch
+
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libnessai_amd_torch.so")
+    lib = load()
+    if not os.path.exists(path):
+        raise RuntimeError(
+            f"nessai_amd torch operators not found at {path}. Build them with `make -C nessai_amd/csrc` "
+            "(or `python -c 'import __graft_entry__ as g; g.build()'`). There is no CPU fallback."
+        )
+    torch.ops.load_library(path)
+    torch.ops.nessai_amd._bind_library(
+        [ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _TORCH_ENTRY_POINTS]
+    )
+    _TORCH_LOADED = True
+
+
 def _check_instance_matrix(lib):
     """The packer lays a spline flow out for the kernel instance ``pack.kernel_bins`` names - the EXACT layout for
     4 / 8 / 10 / 16 bins, the padded 16-bin one otherwise - while the library picks the instance it will launch by

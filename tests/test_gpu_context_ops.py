@@ -418,6 +418,17 @@ def test_embedding_of_indices_outside_the_table():
     assert not dw.any()
 
 
+def test_second_derivatives_are_refused():
+    x, w, b, dy = _group_norm_case((3, 4, 8), 2, torch.float32, torch.float32, "silu")
+    y = ops.group_norm_act(x.requires_grad_(True), 2, w, b, activation="silu")
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(y, [x], dy, create_graph=True)
+    table = randn(5, 4).requires_grad_(True)
+    out = ops.embedding(torch.tensor([1, 2], device=DEV), table)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(out, [table], torch.ones_like(out), create_graph=True)
+
+
 def test_embedding_shapes_views_and_padding():
     w = randn(11, 8, seed=1)
     ids = torch.randint(0, 11, (3, 4, 5), device=DEV)
