@@ -630,6 +630,12 @@ NSA_API int nsa_train_backward(const long long* plan, const int* tables_dev, con
                                float* workspace_dev, int training, const float* g_z_dev,
                                const float* g_logdet_dev, const float* g_log_prob_dev, float* gx_out_dev,
                                void* stream);
+/* The same for a conditional flow whose context is the output of a trainable net: gctx_out_dev [n][C], if not NULL,
+ * receives the gradient with respect to the context rows that the forward call read. */
+NSA_API int nsa_train_backward_ctx(const long long* plan, const int* tables_dev, const float* consts,
+                                   const float* params_dev, float* grads_dev, long long n, float* workspace_dev,
+                                   int training, const float* g_z_dev, const float* g_logdet_dev,
+                                   const float* g_log_prob_dev, float* gx_out_dev, float* gctx_out_dev, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------------
  * Operators around a conditional flow: what a net that makes its context is built from and trained with (the reference

@@ -1231,7 +1231,20 @@ __global__ void tr_gate_backward(long long m, const float* __restrict__ gh, floa
   g[i] = up * tv * sg * (1.0f - sg);
 }
 
-// Gx[row][id_cols[i]] += G[row][i] for i < d_id (the context columns of G carry no gradient anyone needs)
+// gctx[row][c] += G[row][d_id + c]: the context columns of the gradient of a conditional coupling's initial input
+__global__ void tr_add_ctx(int n, int d_id, int C, const float* __restrict__ G, float* __restrict__ gctx) {
+  const long long t = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (t >= (long long)n * C) return;
+  const long long row = t / C;
+  gctx[t] += G[row * (d_id + C) + d_id + (t - row * C)];
+}
+
+__global__ void tr_fill_zero(long long n, float* __restrict__ p) {
+  const long long t = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (t < n) p[t] = 0.0f;
+}
+
+// Gx[row][id_cols[i]] += G[row][i] for i < d_id (the context columns of G: tr_add_ctx)
 __global__ void tr_scatter_add(int n, int d_id, const float* __restrict__ G, int ldg, float* __restrict__ Gx, int ldx,
                                const int* __restrict__ id_cols) {
   const long long t = (long long)blockIdx.x * blockDim.x + threadIdx.x;
@@ -2180,7 +2193,7 @@ static void tr_forward(const long long* plan, const int* tabs, float* params, co
 // ranges_out: the caller sums the per-workgroup gradient copies itself (tr_finish_grads); null: done here
 static void tr_backward(const long long* plan, const int* tabs, const float* params, float* grads,
                         const float* consts, long long n, TrWs& w, int training, hipStream_t s,
-                        TrRanges* ranges_out = nullptr) {
+                        TrRanges* ranges_out = nullptr, float* gctx = nullptr) {
   const int D = (int)plan[0], H = (int)plan[1], L = (int)plan[2], NL = (int)plan[3];
   const int transform = (int)plan[4], K = (int)plan[5], act = (int)plan[6], npf = (int)plan[7];
   const long long rec = plan[9];
@@ -2313,6 +2326,9 @@ static void tr_backward(const long long* plan, const int* tabs, const float* par
           hipLaunchKernelGGL(tr_gate_backward, blocks_for(n * H), dim3(256), 0, s, n * H, w.gh, tl, gl);
           hipLaunchKernelGGL(tr_gemm_tn, tiles(H, C), dim3(256), 0, s, (int)n, H, C, gl, H, w.ctx, C,
                              (const int*)nullptr, ACT_NONE, grads + off[4 + 4 * L + 2 * l], grads + off[5 + 4 * L + 2 * l]);
+          if (gctx != nullptr)  // the context through the gate: d loss / d ctx += gl . Wc
+            hipLaunchKernelGGL(tr_gemm_nn, tiles(n, C), dim3(64), 0, s, (int)n, H, C, gl, H, params + off[4 + 4 * L + 2 * l],
+                               (const float*)nullptr, 0, ACT_NONE, gctx, C, (const int*)nullptr, 1);
           const float* ml = drop ? masks + (long long)l * al4(n * H) : nullptr;
           float* al_ = bn_a + (long long)l * al4(n * H);
           float* vl_ = bn_v + (long long)l * al4(n * H);
@@ -2339,6 +2355,8 @@ static void tr_backward(const long long* plan, const int* tabs, const float* par
         hipLaunchKernelGGL(tr_gemm_nn, tiles(n, W), dim3(64), 0, s, (int)n, H, W, w.gh, H, params + off[0],
                            (const float*)nullptr, 0, ACT_NONE, gxc, W, (const int*)nullptr, 0);
         hipLaunchKernelGGL(tr_scatter_add, blocks_for(n * d_id), dim3(256), 0, s, (int)n, d_id, gxc, W, w.gx, D, id_cols);
+        if (gctx != nullptr)  // ... and through the initial layer, whose last C inputs it is
+          hipLaunchKernelGGL(tr_add_ctx, blocks_for(n * C), dim3(256), 0, s, (int)n, d_id, C, gxc, gctx);
         continue;
       }
       for (int l = L - 1; l >= 0; --l) {
@@ -2601,23 +2619,44 @@ extern "C" NSA_API int nsa_train_forward(const long long* plan, const int* table
   return e == hipSuccess ? NSA_OK : NSA_E_HIP;
 }
 
+static int tr_backward_impl(const long long* plan, const int* tables_dev, const float* consts, const float* params_dev,
+                            float* grads_dev, long long n, float* workspace_dev, int training, const float* g_z_dev,
+                            const float* g_logdet_dev, const float* g_log_prob_dev, float* gx_out_dev,
+                            float* gctx_out_dev, void* stream) {
+  if (!plan || !tables_dev || !consts || !params_dev || !grads_dev || !workspace_dev || n <= 0) return NSA_E_ARG;
+  if (gctx_out_dev != nullptr && plan[13] <= 0) return NSA_E_ARG;  // the flow takes no context
+  hipStream_t s = (hipStream_t)stream;
+  const long long D = plan[0], n_params = plan[8];
+  TrWs w;
+  tr_carve(plan, n, workspace_dev, w);
+  // (a kernel, not hipMemsetAsync: these launches may be captured into a graph)
+  hipLaunchKernelGGL(tr_fill_zero, blocks_for(n_params), dim3(256), 0, s, n_params, grads_dev);
+  if (gctx_out_dev != nullptr)
+    hipLaunchKernelGGL(tr_fill_zero, blocks_for(n * plan[13]), dim3(256), 0, s, n * plan[13], gctx_out_dev);
+  hipLaunchKernelGGL(tr_seed, blocks_for(n * D), dim3(256), 0, s, (int)n, (int)D, w.x, tables_dev + plan[12],
+                     g_z_dev, g_logdet_dev, g_log_prob_dev, consts[6], w.gx, w.gld);
+  hipLaunchKernelGGL(tr_seed_sum, dim3(1), dim3(256), 0, s, (int)n, w.gld, w.scal + 2);
+  tr_backward(plan, tables_dev, params_dev, grads_dev, consts, n, w, training ? 1 : 0, s, nullptr, gctx_out_dev);
+  if (gx_out_dev != nullptr)
+    hipLaunchKernelGGL(tr_copy_rows, blocks_for(n * D), dim3(256), 0, s, n * D, w.gx, gx_out_dev);
+  hipError_t e = hipGetLastError();
+  return e == hipSuccess ? NSA_OK : NSA_E_HIP;
+}
+
 extern "C" NSA_API int nsa_train_backward(const long long* plan, const int* tables_dev, const float* consts,
                                           const float* params_dev, float* grads_dev, long long n,
                                           float* workspace_dev, int training, const float* g_z_dev,
                                           const float* g_logdet_dev, const float* g_log_prob_dev,
                                           float* gx_out_dev, void* stream) {
-  if (!plan || !tables_dev || !consts || !params_dev || !grads_dev || !workspace_dev || n <= 0) return NSA_E_ARG;
-  hipStream_t s = (hipStream_t)stream;
-  const long long D = plan[0], n_params = plan[8];
-  TrWs w;
-  tr_carve(plan, n, workspace_dev, w);
-  (void)hipMemsetAsync(grads_dev, 0, n_params * sizeof(float), s);
-  hipLaunchKernelGGL(tr_seed, blocks_for(n * D), dim3(256), 0, s, (int)n, (int)D, w.x, tables_dev + plan[12],
-                     g_z_dev, g_logdet_dev, g_log_prob_dev, consts[6], w.gx, w.gld);
-  hipLaunchKernelGGL(tr_seed_sum, dim3(1), dim3(256), 0, s, (int)n, w.gld, w.scal + 2);
-  tr_backward(plan, tables_dev, params_dev, grads_dev, consts, n, w, training ? 1 : 0, s);
-  if (gx_out_dev != nullptr)
-    hipLaunchKernelGGL(tr_copy_rows, blocks_for(n * D), dim3(256), 0, s, n * D, w.gx, gx_out_dev);
-  hipError_t e = hipGetLastError();
-  return e == hipSuccess ? NSA_OK : NSA_E_HIP;
+  return tr_backward_impl(plan, tables_dev, consts, params_dev, grads_dev, n, workspace_dev, training, g_z_dev, g_logdet_dev,
+                          g_log_prob_dev, gx_out_dev, nullptr, stream);
+}
+
+extern "C" NSA_API int nsa_train_backward_ctx(const long long* plan, const int* tables_dev, const float* consts,
+                                              const float* params_dev, float* grads_dev, long long n,
+                                              float* workspace_dev, int training, const float* g_z_dev,
+                                              const float* g_logdet_dev, const float* g_log_prob_dev,
+                                              float* gx_out_dev, float* gctx_out_dev, void* stream) {
+  return tr_backward_impl(plan, tables_dev, consts, params_dev, grads_dev, n, workspace_dev, training, g_z_dev, g_logdet_dev,
+                          g_log_prob_dev, gx_out_dev, gctx_out_dev, stream);
 }

@@ -252,7 +252,8 @@ class FlowModel:
         on the validation loss with best-weights restore.  The forward, backward
         and optimiser arithmetic run in the gfx950 kernels (``nessai_amd.train``).
         """
-        from .train import train_flow
+        from .flows import ContextFlow
+        from .train import train_context_flow, train_flow
 
         if not self.initialised:
             self.initialise()
@@ -264,8 +265,9 @@ class FlowModel:
             os.makedirs(output, exist_ok=True)
         if val_size is None:
             val_size = self.training_config["val_size"]
-        history = train_flow(self, samples, max_epochs=max_epochs, patience=patience, val_size=val_size,
-                             weights=weights, conditional=conditional)
+        fit = train_context_flow if isinstance(self.model, ContextFlow) else train_flow
+        history = fit(self, samples, max_epochs=max_epochs, patience=patience, val_size=val_size,
+                      weights=weights, conditional=conditional)
         current_weights_file = os.path.join(output, "model.pt")
         self.save_weights(current_weights_file)
         eval_mode(self.model)

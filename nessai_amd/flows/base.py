@@ -429,14 +429,17 @@ class HipFlow(BaseFlow):
             self._image_key = None
         return tr
 
-    def _wants_grad(self, x):
+    def _wants_grad(self, x, context=None):
         if not torch.is_grad_enabled():
             return False
+        if context is not None and context.requires_grad:
+            return True
         return x.requires_grad or any(p.requires_grad for p in self.parameters())
 
-    def _check_context(self, context, n):
+    def _check_context(self, context, n, trained=False):
         """The ``context`` argument of the B1 methods: ``(n, context_features)`` for a conditional flow (float32 on
-        the flow's device; converted like the inputs), ``None`` for any other - anything else raises."""
+        the flow's device; converted like the inputs), ``None`` for any other - anything else raises.  ``trained``: the
+        context of a ``ContextFlow``, whose net trains with the flow: it keeps its graph."""
         if not self.context_features:
             if context is not None:
                 raise ValueError("this flow was built without context_features: it takes no context")
@@ -450,22 +453,23 @@ class HipFlow(BaseFlow):
                                                                                   tuple(context.shape)))
         if context.dtype == torch.float64:
             raise TypeError(self._FLOAT64_REFUSAL.format(what="The context tensor is float64"))
+        if trained:
+            return context.to(torch.float32).contiguous()
         if context.requires_grad and torch.is_grad_enabled():
-            # (the reverse-mode kernels compute the gradient of the parameters and of x only: a context produced by
-            # a trainable embedding net would train with a zero gradient and no error otherwise)
+            # (a context produced by a trainable embedding net would train with a zero gradient and no error otherwise)
             raise RuntimeError(
                 "the context of a conditional nessai_amd flow carries no gradient: it was given with "
-                "requires_grad=True (an embedding net upstream of the flow would not train); detach it, or "
-                "evaluate under torch.no_grad()"
+                "requires_grad=True (an embedding net upstream of the flow would not train); make the net part of the "
+                "flow (nessai_amd.flows.ContextFlow), detach it, or evaluate under torch.no_grad()"
             )
         return context.detach().to(torch.float32).contiguous()
 
-    def _run(self, x, direction, mode, want_x=True, context=None):
+    def _run(self, x, direction, mode, want_x=True, context=None, context_trained=False):
         stochastic = self.training and _has_dropout(self)  # training mode draws dropout masks, as nflows does
         inner_bn = self.training and _has_inner_batch_norm(self)  # ... and normalises with batch statistics
-        if direction == DIR_FORWARD and (self._wants_grad(x) or stochastic or inner_bn or
-                                         (self.training and _has_norm_layers(self))):
-            return self._run_differentiable(x, mode, want_x, context)
+        if direction == DIR_FORWARD and (self._wants_grad(x, context if context_trained else None) or stochastic or
+                                         inner_bn or (self.training and _has_norm_layers(self))):
+            return self._run_differentiable(x, mode, want_x, context, context_trained)
         if inner_bn:
             raise RuntimeError(
                 "batch_norm_within_layers: the inverse / sampling kernels run on the running statistics (eval mode); "
@@ -482,7 +486,7 @@ class HipFlow(BaseFlow):
                 "mode); call .eval() before inverting or sampling the flow"
             )
         x = self._check_input(x)
-        context = self._check_context(context, x.shape[0])
+        context = self._check_context(context, x.shape[0], context_trained)
         for _ in range(2):
             header, image = self.device_image()
             if context is not None:
@@ -502,9 +506,10 @@ class HipFlow(BaseFlow):
             self.note_f16_overflow()  # raises unless "auto": then the repeat runs in float32
         return (out if want_x else None), ld, self._status
 
-    def _run_differentiable(self, x, mode, want_x, context=None):
+    def _run_differentiable(self, x, mode, want_x, context=None, context_trained=False):
         """Forward direction through the float32 training kernels, recorded by autograd."""
-        context = self._check_context(context, x.shape[0] if isinstance(x, torch.Tensor) and x.dim() == 2 else 0)
+        context = self._check_context(context, x.shape[0] if isinstance(x, torch.Tensor) and x.dim() == 2 else 0,
+                                      context_trained)
         if not isinstance(x, torch.Tensor) or x.device.type != "cuda":
             raise RuntimeError("nessai_amd flows take tensors on a ROCm device; there is no CPU fallback")
         if x.dim() != 2 or x.shape[1] != self.features:

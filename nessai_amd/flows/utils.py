@@ -94,7 +94,8 @@ def _base_distribution(spec, n_inputs, kwargs):
 
 def configure_model(config):
     """A flow from the ``flow_config`` dictionary (``flows/utils.py:208-246``): class from ``flow`` or ``ftype``,
-    the four sizes positionally, everything else by keyword."""
+    the four sizes positionally, everything else by keyword.  ``context_net`` (not in the reference): a net in front of the
+    context (``flows.context.build_context_net``); the flow is then a ``ContextFlow``."""
     cfg = copy.deepcopy(config)
     if not isinstance(cfg["n_inputs"], int):
         raise TypeError("Number of inputs (n_inputs) must be an int")
@@ -109,6 +110,13 @@ def configure_model(config):
     if dist is not None:
         cfg["distribution"] = dist
     sizes = [cfg.pop(k) for k in _POSITIONAL]
+    net = cfg.pop("context_net", None)
+    if net is not None:
+        from .context import ContextFlow, build_context_net
+
+        net = build_context_net(net)
+        cfg.setdefault("context_features", net.features)
+        return ContextFlow(flow_class(*sizes, **cfg), net)
     return flow_class(*sizes, **cfg)
 
 

@@ -15,6 +15,8 @@ the two differentiable ones into autograd:
                                  workspace tensor (``nsa_train_forward``)
 ``nessai_amd::flow_backward``    reverse mode of the above for arbitrary upstream
                                  gradients (``nsa_train_backward``)
+``nessai_amd::flow_backward_ctx``  the same with the gradient of a conditional flow's
+                                 context rows (``nsa_train_backward_ctx``)
 ===============================  =========================================================
 
 Beside the flow stand the operators that a net which makes a flow's context is built from and
@@ -51,6 +53,10 @@ _LIB.define(
 _LIB.define(
     "flow_backward(Tensor(a!) workspace, Tensor flat, int plan, int n, bool training, Tensor? g_z, "
     "Tensor? g_logdet, Tensor? g_log_prob, bool want_gx) -> (Tensor, Tensor)"
+)
+_LIB.define(
+    "flow_backward_ctx(Tensor(a!) workspace, Tensor flat, int plan, int n, bool training, Tensor? g_z, "
+    "Tensor? g_logdet, Tensor? g_log_prob, bool want_gx) -> (Tensor, Tensor, Tensor)"
 )
 
 #: plan handle -> Trainer (the plan, tables and constants of one flow live on the host side)
@@ -133,14 +139,22 @@ def _flow_forward(x, flat, plan, training, want_z, want_logdet, want_log_prob, c
 
 def _flow_backward(workspace, flat, plan, n, training, g_z, g_logdet, g_log_prob, want_gx):
     trainer = _plan(plan)
-    grads, gx = trainer.backward_saved(workspace, int(n), training, g_z, g_logdet, g_log_prob, want_gx)
+    grads, gx, _ = trainer.backward_saved(workspace, int(n), training, g_z, g_logdet, g_log_prob, want_gx)
     return grads, gx if gx is not None else _empty(flat, 0)
+
+
+def _flow_backward_ctx(workspace, flat, plan, n, training, g_z, g_logdet, g_log_prob, want_gx):
+    """``flow_backward`` with the gradient of the context rows of a conditional flow."""
+    trainer = _plan(plan)
+    grads, gx, gctx = trainer.backward_saved(workspace, int(n), training, g_z, g_logdet, g_log_prob, want_gx, want_gctx=True)
+    return grads, gx if gx is not None else _empty(flat, 0), gctx
 
 
 _LIB.impl("flow_run", _flow_run, "CUDA")
 _LIB.impl("flow_run_ctx", _flow_run_ctx, "CUDA")
 _LIB.impl("flow_forward", _flow_forward, "CUDA")
 _LIB.impl("flow_backward", _flow_backward, "CUDA")
+_LIB.impl("flow_backward_ctx", _flow_backward_ctx, "CUDA")
 
 
 # -- shape functions (Meta) -----------------------------------------------------------------
@@ -167,10 +181,15 @@ def _flow_backward_meta(workspace, flat, plan, n, training, g_z, g_logdet, g_log
             flat.new_empty((n, trainer.features)) if want_gx else flat.new_empty((0,)))
 
 
+def _flow_backward_ctx_meta(workspace, flat, plan, n, *rest):
+    return (*_flow_backward_meta(workspace, flat, plan, n, *rest), flat.new_empty((n, _plan(plan).context_features)))
+
+
 _LIB.impl("flow_run", _flow_run_meta, "Meta")
 _LIB.impl("flow_run_ctx", lambda x, context, *rest: _flow_run_meta(x, *rest), "Meta")
 _LIB.impl("flow_forward", _flow_forward_meta, "Meta")
 _LIB.impl("flow_backward", _flow_backward_meta, "Meta")
+_LIB.impl("flow_backward_ctx", _flow_backward_ctx_meta, "Meta")
 
 
 # -- autograd -------------------------------------------------------------------------------
@@ -225,17 +244,19 @@ class FlowFunction(torch.autograd.Function):
         def grad(g, wanted):
             return g.to(torch.float32).contiguous() if (wanted and g is not None) else None
 
-        want_gx = ctx.needs_input_grad[0]
-        grads, gx = torch.ops.nessai_amd.flow_backward(
-            ctx.workspace, trainer.flat, trainer.handle, ctx.n, ctx.training, grad(g_z, want_z),
-            grad(g_ld, want_ld), grad(g_lp, want_lp), bool(want_gx),
-        )
+        want_gx, want_gctx = ctx.needs_input_grad[0], ctx.needs_input_grad[6]
+        args = (ctx.workspace, trainer.flat, trainer.handle, ctx.n, ctx.training, grad(g_z, want_z),
+                grad(g_ld, want_ld), grad(g_lp, want_lp), bool(want_gx))
+        if want_gctx:
+            grads, gx, gctx = torch.ops.nessai_amd.flow_backward_ctx(*args)
+        else:
+            (grads, gx), gctx = torch.ops.nessai_amd.flow_backward(*args), None
         ctx.workspace = None  # a second backward would read activations that were consumed
         per_param = [
             grads[off : off + numel].view(shape) if need else None
             for (off, numel, shape), need in zip(trainer.param_slices, ctx.needs_input_grad[7:])
         ]
-        return (gx if want_gx else None, None, None, None, None, None, None, *per_param)
+        return (gx if want_gx else None, None, None, None, None, None, gctx, *per_param)
 
 
 def _state_version(trainer):

@@ -310,18 +310,19 @@ class Trainer:
             self._actnorm_initialised()
         return z, ld, lp, ws
 
-    def backward_saved(self, ws, n, training, g_z=None, g_logdet=None, g_log_prob=None, want_gx=False):
-        """Gradients of every trainable float (a fresh flat tensor) and optionally of the input."""
+    def backward_saved(self, ws, n, training, g_z=None, g_logdet=None, g_log_prob=None, want_gx=False, want_gctx=False):
+        """Gradients of every trainable float (a fresh flat tensor) and optionally of the input and of the context."""
         grads = torch.empty(self.n_params, dtype=torch.float32, device=self.device)
         gx = torch.empty((n, self.features), dtype=torch.float32, device=self.device) if want_gx else None
+        gctx = torch.empty((n, self.context_features), dtype=torch.float32, device=self.device) if want_gctx else None
         stream = torch.cuda.current_stream(self.device).cuda_stream
-        rc = lib.load().nsa_train_backward(
+        rc = lib.load().nsa_train_backward_ctx(
             self.plan, lib.ptr(self.tables), self.consts, lib.ptr(self.flat), lib.ptr(grads), n, lib.ptr(ws),
-            1 if training else 0, lib.ptr(g_z), lib.ptr(g_logdet), lib.ptr(g_log_prob), lib.ptr(gx),
+            1 if training else 0, lib.ptr(g_z), lib.ptr(g_logdet), lib.ptr(g_log_prob), lib.ptr(gx), lib.ptr(gctx),
             lib.c_void_p(stream),
         )
-        lib.check(rc, "nsa_train_backward")
-        return grads, gx
+        lib.check(rc, "nsa_train_backward_ctx")
+        return grads, gx, gctx
 
     def _count_training_pass(self):
         for bn in self._inner_bns:  # torch's BatchNorm1d counts its training-mode passes (a state_dict entry)
@@ -455,22 +456,106 @@ def _training_kernels(deterministic):
                 os.environ["NESSAI_AMD_TRAIN_FUSED"] = before
 
 
-def train_flow(flow_model, samples, max_epochs=None, patience=None, val_size=None, weights=None, conditional=None):
-    tc = flow_model.training_config
-    trainer = get_trainer(flow_model)
-    trainer.lr = trainer.base_lr
-    # Gaussian noise added to every training minibatch (flowmodel/base.py:424-425, 596-605)
-    noise_scale = None
+def _noise_scale(tc, samples):
+    """Gaussian noise added to every training minibatch (flowmodel/base.py:424-425, 596-605); ``None``: none."""
     if tc.get("noise_type") == "adaptive":
         from scipy.spatial import distance
 
         d = distance.cdist(samples, samples, "euclidean")  # utils/distance.py:10-30
         d[d == 0] = np.nan
-        noise_scale = float(tc["noise_scale"] * np.mean(np.nanmin(d, axis=1)))
-    elif tc.get("noise_type") == "constant":
-        noise_scale = float(tc["noise_scale"])
-    elif tc.get("noise_type"):
+        return float(tc["noise_scale"] * np.mean(np.nanmin(d, axis=1)))
+    if tc.get("noise_type") == "constant":
+        return float(tc["noise_scale"])
+    if tc.get("noise_type"):
         raise ValueError(f"Unknown noise type: {tc['noise_type']}")
+    return None
+
+
+def get_context_optimiser(flow_model):
+    """The torch optimiser of a ``ContextFlow`` - the reference's own (``FlowModel.get_optimiser``, flowmodel/base.py:105-135)
+    over the flow's and the net's parameters; a new one whenever the FlowModel dropped its handle (``reset_model``)."""
+    if flow_model._trainer is None:
+        tc = flow_model.training_config
+        name = (tc.get("optimiser") or "adamw").lower()
+        classes = {"adamw": (torch.optim.AdamW, {}), "adam": (torch.optim.Adam, dict(weight_decay=1e-6)), "sgd": (torch.optim.SGD, {})}
+        if name not in classes:
+            raise NotImplementedError(f"optimiser {name!r} is not supported (adamw, adam, sgd)")
+        make, defaults = classes[name]
+        flow_model._trainer = make(flow_model.model.parameters(), **{"lr": tc["lr"], **defaults, **(tc.get("optimiser_kwargs") or {})})
+    return flow_model._trainer
+
+
+def train_context_flow(flow_model, samples, max_epochs=None, patience=None, val_size=None, weights=None, conditional=None):
+    """``train_flow`` of a flow with a net in front of its context: the reference's loop (flowmodel/base.py:400-452) over the
+    parameters of both, through autograd.  The flow's forward and backward passes are the training kernels, the net's its own
+    operators, the clip over all gradients ``ops.clip_grad_norm_``, the update torch's optimiser."""
+    from . import ops
+
+    tc = flow_model.training_config
+    if conditional is None:
+        raise ValueError("a flow with a context net trains on conditional inputs (conditional=...)")
+    noise_scale = _noise_scale(tc, samples)
+    validate = val_size != 0.0
+    (x_train, c_train), (x_val, c_val), batch_size = flow_model.prep_data(
+        samples, val_size=val_size, batch_size=tc["batch_size"], weights=weights, conditional=conditional
+    )
+    model = flow_model.model
+    optimiser = get_context_optimiser(flow_model)
+    max_epochs = tc["max_epochs"] if max_epochs is None else max_epochs
+    patience = tc["patience"] if patience is None else patience
+    base_lrs = [(tc.get("optimiser_kwargs") or {}).get("lr", tc["lr"])] * len(optimiser.param_groups)
+    has_val = bool(validate and len(x_val))
+    parameters, n_train = list(model.parameters()), x_train.shape[0]
+    bounds = [(a, min(a + batch_size, n_train)) for a in range(0, n_train, batch_size)]
+    best_epoch, best_val_loss = 0, np.inf
+    best = {k: v.detach().clone() for k, v in model.state_dict().items()}
+    history = dict(loss=[], val_loss=[])
+    with _training_kernels(tc.get("deterministic")), torch.enable_grad():
+        for epoch in range(1, max_epochs + 1):
+            for group, lr in zip(optimiser.param_groups, base_lrs):
+                group["lr"] = lr * (0.5 * (1.0 + math.cos(math.pi * (epoch - 1) / max_epochs)) if tc.get("annealing") else 1.0)
+            model.train()
+            perm = torch.randperm(n_train).to(x_train.device)
+            losses = torch.zeros(2, dtype=torch.float32, device=x_train.device)
+            for a, b in bounds:
+                rows = perm[a:b]
+                x = x_train[rows]
+                if noise_scale:
+                    x = x + noise_scale * torch.randn_like(x)
+                optimiser.zero_grad()
+                loss = -model.log_prob(x, context=c_train[rows]).mean()
+                loss.backward()
+                if tc["clip_grad_norm"]:
+                    ops.clip_grad_norm_(parameters, tc["clip_grad_norm"])
+                optimiser.step()
+                losses[0] += loss.detach()
+            model.eval()
+            if has_val:
+                with torch.no_grad():
+                    trainer = model.flow.trainer()
+                    trainer.losses.zero_()
+                    trainer.evaluate(x_val, context=model.net(c_val))
+                    losses[1] = trainer.losses[0]
+            loss, val_loss = (float(v) for v in losses.tolist())  # the epoch's one sync
+            history["loss"].append(loss / len(bounds))
+            history["val_loss"].append(val_loss if has_val else np.nan)
+            if validate and val_loss < best_val_loss and has_val:
+                best_epoch, best_val_loss = epoch, val_loss
+                best = {k: v.detach().clone() for k, v in model.state_dict().items()}
+            if validate and epoch - best_epoch > patience:
+                break
+    if validate:
+        model.load_state_dict(best)
+    model.flow._image_key = None  # (batch norm's statistics change behind torch's version counters)
+    model.eval()
+    return history
+
+
+def train_flow(flow_model, samples, max_epochs=None, patience=None, val_size=None, weights=None, conditional=None):
+    tc = flow_model.training_config
+    trainer = get_trainer(flow_model)
+    trainer.lr = trainer.base_lr
+    noise_scale = _noise_scale(tc, samples)
     model = flow_model.model
     validate = val_size != 0.0
     train_data, val_data, batch_size = flow_model.prep_data(
