@@ -650,8 +650,9 @@ enum { NSA_FN_NONE = -1, NSA_FN_RELU = 0, NSA_FN_TANH = 1, NSA_FN_SILU = 2 };   
 /* norm_out_dev[0] = the norm over all elements of `count` tensors (tensors[i]: device pointer, sizes[i] contiguous
  * elements of type dtypes[i]; the three arrays are host memory and are read before the call returns).  A tensor listed
  * twice counts twice.  nsa_grad_clip then multiplies every element by min(1, max_norm / (norm + 1e-6)); there two
- * tensors must not overlap (NSA_E_ARG).  workspace_dev: nsa_grad_norm_workspace(count) bytes, 8-byte aligned. */
-NSA_API size_t nsa_grad_norm_workspace(int count);
+ * tensors must not overlap (NSA_E_ARG).  workspace_dev: nsa_grad_norm_workspace(count, elements of all tensors) bytes,
+ * 8-byte aligned. */
+NSA_API size_t nsa_grad_norm_workspace(int count, long long elements);
 NSA_API int nsa_grad_norm(int count, void* const* tensors, const long long* sizes, const int* dtypes, int kind,
                           void* workspace_dev, size_t workspace_bytes, float* norm_out_dev, void* stream);
 NSA_API int nsa_grad_clip(int count, void* const* tensors, const long long* sizes, const int* dtypes, int kind,

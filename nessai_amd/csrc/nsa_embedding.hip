@@ -378,14 +378,18 @@ int emb_vector(int width, int bytes, uintptr_t addresses) {
   return v;
 }
 
-// lanes of a team: a power of two up to a wave that leaves few lanes idle in a row of `vectors` accesses
+// Lanes of a team, a power of two.  A short row: one access of each lane.  A longer one: eight lanes or more (128 bytes side
+// by side), as many as leave at most an eighth of them idle in its last round; 40 accesses, for one, are five rounds of 8.
 int emb_lanes(int vectors) {
   int best = 1;
-  for (int l = 1; l <= 64; l <<= 1) {
-    const int rounds = (vectors + l - 1) / l;
-    if (rounds * l * 8 <= vectors * 9 || l <= vectors / 2) best = l;  // at most an eighth idle, or two rounds and more
+  if (vectors <= 8) {
+    while (best < vectors) best *= 2;
+    return best;
   }
-  return vectors == 1 ? 1 : best;
+  best = 8;
+  for (int l = 16; l <= 64; l *= 2)
+    if ((vectors + l - 1) / l * l * 8 <= vectors * 9) best = l;
+  return best;
 }
 
 int emb_passes(long long vocab) {  // 8 bits each; the largest key is `vocab` itself
@@ -426,7 +430,9 @@ EmbFew emb_few_plan(long long n, long long vocab, int width, int bytes) {
   while (f.lanes < 64 && f.lanes < vectors) f.lanes *= 2;
   f.slabs = (vectors + f.lanes - 1) / f.lanes;
   const long long step = (long long)(EMB_THREADS / f.lanes) * EMB_FEW_AHEAD;  // tokens of a workgroup in flight
-  const long long blocks = std::max(1LL, std::min(1024LL / f.slabs + 1, n / step));
+  // as many workgroups as the 256 compute units hold at once, 160 KB of LDS each: one more would run alone behind them
+  const long long fit = 256 * std::min(8LL, 160 * 1024 / (vocab * EMB_THREADS * f.words * 4));
+  const long long blocks = std::max(1LL, std::min(fit / f.slabs, n / step));
   f.share = (n + blocks - 1) / blocks;
   f.blocks = (int)((n + f.share - 1) / f.share);
   return f;

@@ -16,15 +16,16 @@
 
 #include "nsa_elem.h"
 
-#define NG_RUNS 224          // runs per launch: 2 x 8 bytes each, inside the 4 KB of a kernel's arguments
+#define NG_RUNS 320          // runs per launch: 8 + 4 bytes each, inside the 4 KB of a kernel's arguments
+#define NG_MOST (1LL << 31)  // elements per launch: their numbers fit 32 bits (a longer run is cut)
 #define NG_THREADS 256
 #define NG_BLOCKS 2048       // workgroups of a launch at most: 8 per compute unit ...
 #define NG_BLOCKS_MIN 128    // ... and fewer where there are many launches: every partial sum is read by all of them
 #define NG_SHARE 4096        // elements of a workgroup's share: a multiple of this
 
 struct NgRuns {
-  long long first[NG_RUNS + 1];  // elements in front of run k
   void* ptr[NG_RUNS];
+  uint32_t first[NG_RUNS + 1];  // elements in front of run k
   int count;
 };
 
@@ -64,7 +65,7 @@ __device__ __forceinline__ double ng_block_join(double s) {  // the sum on every
 
 // the elements [lo, hi) of the launch, run by run: f(pointer, length), each a contiguous piece
 template <typename F>
-__device__ __forceinline__ void ng_pieces(const NgRuns& r, long long lo, long long hi, F f) {
+__device__ __forceinline__ void ng_pieces(const NgRuns& r, uint32_t lo, uint32_t hi, F f) {
   int a = 0, b = r.count;  // first[a] <= lo < first[b]
   while (b - a > 1) {
     const int m = (a + b) >> 1;
@@ -72,7 +73,7 @@ __device__ __forceinline__ void ng_pieces(const NgRuns& r, long long lo, long lo
     else b = m;
   }
   while (lo < hi) {
-    const long long end = r.first[a + 1] < hi ? r.first[a + 1] : hi;
+    const uint32_t end = r.first[a + 1] < hi ? r.first[a + 1] : hi;
     f(r.ptr[a], lo - r.first[a], end - lo);
     lo = end;
     ++a;
@@ -99,12 +100,11 @@ __device__ __forceinline__ void ng_piece(T* p, long long len, ONE one, WIDE wide
 }
 
 template <typename T, int KIND>
-__global__ void __launch_bounds__(NG_THREADS) ng_partial(NgRuns r, long long share, double* __restrict__ partial) {
+__global__ void __launch_bounds__(NG_THREADS) ng_partial(NgRuns r, uint32_t share, double* __restrict__ partial) {
   constexpr int V = 16 / sizeof(T);
   NgAcc<KIND> acc;
-  const long long lo = blockIdx.x * share;
-  const long long hi = lo + share < r.first[r.count] ? lo + share : r.first[r.count];
-  ng_pieces(r, lo, hi, [&](const void* base, long long at, long long len) {
+  const uint32_t lo = blockIdx.x * share, total = r.first[r.count], hi = total - lo < share ? total : lo + share;
+  ng_pieces(r, lo, hi, [&](const void* base, uint32_t at, uint32_t len) {
     ng_piece((const T*)base + at, len, [&](const T* p) { acc.add((float)*p, 0); },
              [&](const T* p, int count) {
                float v[NG_AHEAD][V];
@@ -147,7 +147,7 @@ __device__ __forceinline__ float ng_factor(float norm, float max_norm) {
 // Every workgroup adds up the partial sums by itself (at most a few thousand values out of the L2 cache, in the same
 // order everywhere) instead of waiting for one that does: one launch less between the norm and the product.
 template <typename T, int KIND>
-__global__ void __launch_bounds__(NG_THREADS) ng_scale(NgRuns r, long long share, const double* __restrict__ partial,
+__global__ void __launch_bounds__(NG_THREADS) ng_scale(NgRuns r, uint32_t share, const double* __restrict__ partial,
                                                        int n_partial, float max_norm, float* __restrict__ norm_out) {
   constexpr int V = 16 / sizeof(T);
   const float norm = ng_total<KIND>(partial, n_partial);
@@ -155,9 +155,9 @@ __global__ void __launch_bounds__(NG_THREADS) ng_scale(NgRuns r, long long share
   const float f = ng_factor(norm, max_norm);
   if (f == 1.0f) return;  // (a product by one changes nothing)
   // the shares from the last to the first: what the norm read last is the likeliest to be in a cache still
-  const long long lo = (gridDim.x - 1 - blockIdx.x) * share;
-  const long long hi = lo + share < r.first[r.count] ? lo + share : r.first[r.count];
-  ng_pieces(r, lo, hi, [&](void* base, long long at, long long len) {
+  const uint32_t lo = (gridDim.x - 1 - blockIdx.x) * share, total = r.first[r.count];
+  const uint32_t hi = total - lo < share ? total : lo + share;
+  ng_pieces(r, lo, hi, [&](void* base, uint32_t at, uint32_t len) {
     ng_piece((T*)base + at, len, [&](T* p) { *p = (T)((float)*p * f); },
              [&](T* p, int count) {
                float v[NG_AHEAD][V];
@@ -261,28 +261,36 @@ bool ng_runs(int count, void* const* tensors, const long long* sizes, const int*
 struct Launch {
   NgRuns r;
   int dtype, blocks;
-  long long share;
+  uint32_t share;
 };
 
 void ng_launches(const std::vector<Run>& runs, std::vector<Launch>& out) {
   out.clear();
-  for (size_t i = 0; i < runs.size();) {
+  size_t i = 0;
+  long long done = 0;  // of run i
+  while (i < runs.size()) {
     Launch l;
     l.dtype = runs[i].dtype;
     l.r.count = 0;
     l.r.first[0] = 0;
     while (i < runs.size() && l.r.count < NG_RUNS && runs[i].dtype == l.dtype) {
-      l.r.ptr[l.r.count] = runs[i].ptr;
-      l.r.first[l.r.count + 1] = l.r.first[l.r.count] + runs[i].n;
+      const long long room = NG_MOST - l.r.first[l.r.count], n = std::min(runs[i].n - done, room);
+      if (n == 0) break;
+      l.r.ptr[l.r.count] = runs[i].ptr + done * nsa_elem_bytes(l.dtype);
+      l.r.first[l.r.count + 1] = (uint32_t)(l.r.first[l.r.count] + n);
       ++l.r.count;
-      ++i;
+      done += n;
+      if (done == runs[i].n) {
+        ++i;
+        done = 0;
+      }
     }
     out.push_back(l);
   }
   const int blocks = std::max(NG_BLOCKS_MIN, 2 * NG_BLOCKS / (int)(out.size() + 1));
   for (Launch& l : out) {
     const long long total = l.r.first[l.r.count], shares = (total + NG_SHARE - 1) / NG_SHARE;
-    l.share = (shares + blocks - 1) / blocks * NG_SHARE;
+    l.share = (uint32_t)((shares + blocks - 1) / blocks * NG_SHARE);
     l.blocks = (int)((total + l.share - 1) / l.share);
   }
 }
@@ -313,14 +321,15 @@ int ng_run(const char* what, int count, void* const* tensors, const long long* s
     if ((uintptr_t)tensors[i] % nsa_elem_bytes(dtypes[i]) != 0)
       return nsa_fail(NSA_E_ARG, "%s: tensor %d is not aligned to its elements", what, i);
   }
-  if (workspace_bytes < nsa_grad_norm_workspace(count))
-    return nsa_fail(NSA_E_ARG, "%s: workspace too small", what);
   try {
     std::vector<Run> runs;
     std::vector<Launch> launches;
     const bool apart = ng_runs(count, tensors, sizes, dtypes, runs);
     if (clip && !apart) return nsa_fail(NSA_E_ARG, "%s: two gradients overlap in memory", what);
     ng_launches(runs, launches);
+    size_t partials = 0;
+    for (const Launch& l : launches) partials += l.blocks;
+    if (workspace_bytes < partials * sizeof(double)) return nsa_fail(NSA_E_ARG, "%s: workspace too small", what);
     if (launches.size() == 1 && launches[0].r.first[launches[0].r.count] <= NG_SMALL) {
       const Launch& l = launches[0];
       NG_DISPATCH(l.dtype, ng_small, dim3(1), dim3(NG_SMALL_THREADS), 0, s, l.r, clip ? 1 : 0, max_norm, norm_out)
@@ -356,10 +365,11 @@ int ng_run(const char* what, int count, void* const* tensors, const long long* s
 
 }  // namespace
 
-extern "C" NSA_API size_t nsa_grad_norm_workspace(int count) {
-  // one partial sum per workgroup of every launch; the three types make at most two launches more
-  const size_t launches = (size_t)(count > 0 ? count : 0) / NG_RUNS + 3;
-  return launches * NG_BLOCKS * sizeof(double);
+// One partial sum per workgroup.  `count` tensors make at most count / NG_RUNS + 3 launches (one not full for each type) and
+// one more for every NG_MOST elements; with L launches a launch has at most max(NG_BLOCKS_MIN, 2 NG_BLOCKS / (L + 1)) groups.
+extern "C" NSA_API size_t nsa_grad_norm_workspace(int count, long long elements) {
+  const size_t launches = (size_t)std::max(count, 0) / NG_RUNS + 3 + (size_t)(std::max(elements, 0LL) / NG_MOST);
+  return (launches * NG_BLOCKS_MIN + 2 * NG_BLOCKS) * sizeof(double);
 }
 
 extern "C" NSA_API int nsa_grad_norm(int count, void* const* tensors, const long long* sizes, const int* dtypes, int kind,

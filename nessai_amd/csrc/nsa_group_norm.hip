@@ -105,6 +105,21 @@ __device__ __forceinline__ GnPlace gn_place(const GnShape& s) {
   return p;
 }
 
+// f(i, channel, index of its (sample, group)) for the V channels from c of the slab on: one division, not V
+template <int V, typename F>
+__device__ __forceinline__ void gn_group_of(const GnShape& s, const GnPlace& p, int c, F f) {
+  const int first = p.slab * s.width + c;
+  int g = first / s.cpg, in = first - g * s.cpg;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    f(i, first + i, p.n * s.groups + g);
+    if (++in == s.cpg) {
+      in = 0;
+      ++g;
+    }
+  }
+}
+
 // This thread's positions of the chunk, GN_AHEAD at a time: ask(slot, offset) for all of them, then use(slot, offset).  The
 // offset is that of the thread's channels c at a position.
 #define GN_AHEAD 4
@@ -240,14 +255,12 @@ __global__ void __launch_bounds__(GN_THREADS) gn_apply(GnShape s, const T* __res
     const int c = (t * s.vecs + p.j) * V;
     if (c >= s.width) break;
     float mu[V], rs[V], w[V], b[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int ch = p.slab * s.width + c + i;
-      mu[i] = mean[p.n * s.groups + ch / s.cpg];
-      rs[i] = rstd[p.n * s.groups + ch / s.cpg];
+    gn_group_of<V>(s, p, c, [&](int i, int ch, long long k) {
+      mu[i] = mean[k];
+      rs[i] = rstd[k];
       w[i] = gn_param<T>(q.w, q.f32, ch, 1.0f);
       b[i] = gn_param<T>(q.b, q.f32, ch, 0.0f);
-    }
+    });
     NsaPack<T, V> px[GN_AHEAD];
     gn_positions(s, p, c, [&](int k, long long at) { px[k] = *reinterpret_cast<const NsaPack<T, V>*>(x + at); },
                  [&](int k, long long at) {
@@ -277,14 +290,12 @@ __global__ void __launch_bounds__(GN_THREADS) gn_sums(GnShape s, const T* __rest
     for (int i = 0; i < V; ++i) s1[i] = s2[i] = 0.0f;
     if (p.active && c < s.width) {
       float mu[V], rs[V], w[V], b[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int ch = p.slab * s.width + c + i;
-        mu[i] = mean[p.n * s.groups + ch / s.cpg];
-        rs[i] = rstd[p.n * s.groups + ch / s.cpg];
+      gn_group_of<V>(s, p, c, [&](int i, int ch, long long k) {
+        mu[i] = mean[k];
+        rs[i] = rstd[k];
         w[i] = gn_param<T>(q.w, q.f32, ch, 1.0f);
         b[i] = gn_param<T>(q.b, q.f32, ch, 0.0f);
-      }
+      });
       NsaPack<T, V> px[GN_AHEAD], pd[GN_AHEAD];
       gn_positions(s, p, c,
                    [&](int k, long long at) {
@@ -379,17 +390,14 @@ __global__ void __launch_bounds__(GN_THREADS) gn_dx(GnShape s, const T* __restri
     const int c = (t * s.vecs + p.j) * V;
     if (c >= s.width) break;
     float mu[V], rs[V], w[V], b[V], ga[V], gb[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int ch = p.slab * s.width + c + i;
-      const long long k = p.n * s.groups + ch / s.cpg;
+    gn_group_of<V>(s, p, c, [&](int i, int ch, long long k) {
       mu[i] = mean[k];
       rs[i] = rstd[k];
       ga[i] = ab[k].x;
       gb[i] = ab[k].y;
       w[i] = gn_param<T>(q.w, q.f32, ch, 1.0f);
       b[i] = gn_param<T>(q.b, q.f32, ch, 0.0f);
-    }
+    });
     NsaPack<T, V> px[GN_AHEAD], pd[GN_AHEAD];
     gn_positions(s, p, c,
                  [&](int k, long long at) {

@@ -265,13 +265,15 @@ Tensor norm_call(const std::vector<Tensor>& tensors, int64_t kind, bool clip, do
   std::vector<void*> places(count);
   std::vector<long long> sizes(count);
   std::vector<int> codes(count);
+  long long elements = 0;
   for (int i = 0; i < count; ++i) {
     places[i] = const_cast<void*>(tensors[i].const_data_ptr());
     sizes[i] = tensors[i].numel();
+    elements += sizes[i];
     codes[i] = dtype_code(tensors[i], "gradients");
   }
   Tensor out = at::empty({}, tensors[0].options().dtype(at::kFloat));
-  const size_t size = g_entry.grad_norm_workspace(count);
+  const size_t size = g_entry.grad_norm_workspace(count, elements);
   const Tensor ws = workspace(out, size);
   if (clip)
     check(g_entry.grad_clip(count, places.data(), sizes.data(), codes.data(), kind, (float)max_norm, ws.mutable_data_ptr(),

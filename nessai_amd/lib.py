@@ -181,7 +181,7 @@ SIGNATURES = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
          c_void_p, c_void_p, c_void_p],
     ),
-    "nsa_grad_norm_workspace": (c_size_t, [c_int]),
+    "nsa_grad_norm_workspace": (c_size_t, [c_int, c_ll]),
     "nsa_grad_norm": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_void_p, c_void_p]),
     "nsa_grad_clip": (
         c_int,

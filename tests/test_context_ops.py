@@ -81,8 +81,8 @@ def _norm_args(places, sizes, codes):
 def test_entry_points_check_their_arguments_before_anything_is_launched():
     L = lib.load()
     ws, out = 4096, 8192  # addresses that no call below reaches
-    size = L.nsa_grad_norm_workspace(2)
-    assert L.nsa_grad_norm_workspace(10_000) >= size > 0
+    size = L.nsa_grad_norm_workspace(2, 1000)
+    assert L.nsa_grad_norm_workspace(10_000, 10**12) >= size > 0
     for places, sizes, codes, kind, max_norm, bytes_, message in (
         ((16, 32), (4, 5), (0, 7), 2, 1.0, size, b"unknown type"),
         ((16, 32), (4, -1), (0, 0), 2, 1.0, size, b"bad tensor"),
@@ -91,7 +91,7 @@ def test_entry_points_check_their_arguments_before_anything_is_launched():
         ((16, 32), (4, 5), (0, 0), 9, 1.0, size, b"unknown norm"),
         ((16, 32), (4, 5), (0, 0), 2, -1.0, size, b"max_norm"),
         ((16, 32), (4, 5), (0, 0), 2, math.nan, size, b"max_norm"),
-        ((16, 32), (4, 5), (0, 0), 2, 1.0, size - 1, b"workspace"),
+        ((64, 128), (4, 5), (0, 0), 2, 1.0, 7, b"workspace"),
         ((16, 28), (4, 5), (0, 0), 2, 1.0, size, b"overlap"),
         ((16, 16), (4, 4), (0, 0), 2, 1.0, size, b"overlap"),
         ((16, 24), (2, 20), (0, 1), 2, 1.0, 0, b"workspace"),
