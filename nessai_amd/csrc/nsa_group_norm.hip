@@ -5,6 +5,14 @@
 //   backward, dz = dy act'(z):   db[c] = sum_{n,l} dz     dw[c] = sum_{n,l} dz xh
 //     A = 1/m sum_group w dz     B = 1/m sum_group w dz xh     dx = r (w dz - A - xh B)
 //
+// Three ways, by the size of a sample (gn_rows, gn_tile_threads):
+//   rows of a power of two of channels     one pass, shuffles:    200003 x 128 float32, 32 groups: forward 40 us (205 MB at
+//                                          5.1 TB/s), with the backward pass 106 us (512 MB at 4.8 TB/s); as tiles 60 and 197
+//   up to 8192 values (backward 4096)      one pass through LDS:  1000 x 64 x 128 float32: forward 21 us
+//   longer samples                         statistics, their join, then the values once more: 16 x 4096 x 256 bfloat16
+//                                          (34 MB): 11 + 4 + 19 us, the second reading out of the last-level cache
+// A large copy on this card runs at 5.07 TB/s.
+//
 // Memory-bound.  In a channels-last array the channels of a group lie side by side and its positions far apart, so a
 // workgroup takes whole rows (all channels, or a slab of whole groups where a row is too wide) of a stretch of positions:
 // its accesses are contiguous whatever the groups are.  A thread keeps to V neighbouring channels and walks over positions.
@@ -893,17 +901,36 @@ bool gn_rows(const GnShape& s, int v, GnRows& q) {
   return true;
 }
 
-// An upper bound that does not ask for the addresses: chunks do not grow with a narrower access by more than the rows do
+size_t gn_tile_lds(const GnTile& q, int threads, bool backward) {
+  const size_t stat = (size_t)q.per * q.groups * sizeof(float2);
+  if (!backward) return (size_t)threads * GN_EACH * 4 + stat;
+  return (size_t)threads * GN_EACH * 8 + stat + (size_t)(q.channels + 1) / 2 * 8 +
+         (size_t)std::max(threads, q.channels) * sizeof(float2);
+}
+
+// Whether the one-pass tiles take these samples, with 256 threads (4096 values) or, forward, 512 (8192); 0: they do not.
+// 1000 samples of 8192 float32 values: 21 us in a tile, 30 in the three passes below; of 16384 bfloat16 values the passes are
+// faster (2000 samples: 58 us against 86 in tiles of that size, of which two fit a compute unit).  Backward, where a tile
+// needs twice the LDS, larger ones do not pay.
+int gn_tile_threads(long long samples, long long length, int channels, int groups, int v, bool backward, GnTile& q) {
+  for (int threads = 256; threads <= (backward ? 256 : 512); threads *= 2)
+    if (gn_tile(samples, length, channels, groups, v, threads * GN_EACH, q) && gn_tile_lds(q, threads, backward) <= GN_LDS)
+      return threads;
+  return 0;
+}
+
+// An upper bound that does not ask for the addresses: where the one-pass kernels take the samples (whatever the access width),
+// the records of the backward pass; otherwise the chunks' sums at the widest access that any address allows.
 size_t gn_workspace(long long samples, long long length, int channels, int groups, int bytes, bool backward) {
+  GnTile q;
+  if (gn_tile_threads(samples, length, channels, groups, 1, backward, q) != 0)
+    return 256 + (backward ? (size_t)std::min(samples, (long long)GN_TILE_BLOCKS) * channels * sizeof(float2) : 0);
   size_t most = 0;
   for (int align = bytes; align <= 16; align *= 2) {
     int v;
     const GnShape s = gn_shape(samples, length, channels, groups, bytes, (uintptr_t)align, v);
-    const size_t parts = (size_t)s.samples * s.chunks * (backward ? s.channels : s.groups) * sizeof(float2);
-    most = std::max(most, parts);
+    most = std::max(most, (size_t)s.samples * s.chunks * (backward ? s.channels : s.groups) * sizeof(float2));
   }
-  if (backward && length * channels <= 256 * GN_EACH)  // the one-pass kernels' records
-    most = std::max(most, (size_t)std::min(samples, (long long)GN_TILE_BLOCKS) * channels * sizeof(float2));
   return most + (backward ? (size_t)samples * groups * sizeof(float2) : 0) + 256;
 }
 
@@ -956,16 +983,14 @@ void gn_forward(const GnShape& s, const void* x, GnParams q, float eps, int act,
             (const T*)x, q, eps, mean, rstd, (T*)y)
     return;
   }
-  GnTile q_;
-  for (int threads = 256; threads <= 1024; threads *= 4) {
-    if (!gn_tile(s.samples, s.length, s.channels, s.groups, V, threads * GN_EACH, q_)) continue;
-    const size_t lds = (size_t)threads * GN_EACH * 4 + (size_t)q_.per * q_.groups * sizeof(float2);
-    if (lds > GN_LDS) break;
-    const dim3 tiles((unsigned)((s.samples + q_.per - 1) / q_.per));
+  GnTile tile;
+  if (const int threads = gn_tile_threads(s.samples, s.length, s.channels, s.groups, V, false, tile)) {
+    const size_t lds = gn_tile_lds(tile, threads, false);
+    const dim3 tiles((unsigned)((s.samples + tile.per - 1) / tile.per));
     if (threads == 256) {
-      GN_TILE_ACTS(act, gn_tile_forward, T, V, 256, lds, tiles, dim3(256), lds, st, q_, (const T*)x, q, eps, mean, rstd, (T*)y)
+      GN_TILE_ACTS(act, gn_tile_forward, T, V, 256, lds, tiles, dim3(256), lds, st, tile, (const T*)x, q, eps, mean, rstd, (T*)y)
     } else {
-      GN_TILE_ACTS(act, gn_tile_forward, T, V, 1024, lds, tiles, dim3(1024), lds, st, q_, (const T*)x, q, eps, mean, rstd, (T*)y)
+      GN_TILE_ACTS(act, gn_tile_forward, T, V, 512, lds, tiles, dim3(512), lds, st, tile, (const T*)x, q, eps, mean, rstd, (T*)y)
     }
     return;
   }
@@ -994,16 +1019,13 @@ void gn_backward(const GnShape& s, const void* x, const void* dy, GnParams q, in
             mean, rstd, (T*)dx, sums ? part : nullptr)
     return params(blocks, s.channels);
   }
-  GnTile q_;
-  if (gn_tile(s.samples, s.length, s.channels, s.groups, V, 256 * GN_EACH, q_)) {
-    const size_t lds = (size_t)256 * GN_EACH * 8 + (size_t)q_.per * q_.groups * sizeof(float2) +
-                       (size_t)(s.channels + 1) / 2 * 8 + (size_t)std::max(256, s.channels) * sizeof(float2);
-    if (lds <= GN_LDS) {
-      const int blocks = (int)std::min((s.samples + q_.per - 1) / q_.per, (long long)GN_TILE_BLOCKS);
-      GN_TILE_ACTS(act, gn_tile_backward, T, V, 256, lds, dim3(blocks), dim3(256), lds, st, q_, (const T*)x, (const T*)dy, q,
-                   mean, rstd, (T*)dx, sums ? part : nullptr)
-      return params(blocks, s.channels);
-    }
+  GnTile tile;
+  if (gn_tile_threads(s.samples, s.length, s.channels, s.groups, V, true, tile) != 0) {
+    const size_t lds = gn_tile_lds(tile, 256, true);
+    const int blocks = (int)std::min((s.samples + tile.per - 1) / tile.per, (long long)GN_TILE_BLOCKS);
+    GN_TILE_ACTS(act, gn_tile_backward, T, V, 256, lds, dim3(blocks), dim3(256), lds, st, tile, (const T*)x, (const T*)dy, q,
+                 mean, rstd, (T*)dx, sums ? part : nullptr)
+    return params(blocks, s.channels);
   }
   const dim3 grid((unsigned)(s.samples * s.slabs * s.chunks)), block(GN_THREADS);
   GN_ACTS(act, gn_sums, T, V, grid, block, 0, st, s, (const T*)x, (const T*)dy, q, mean, rstd, part)
@@ -1077,8 +1099,10 @@ extern "C" NSA_API int nsa_group_norm_backward(long long samples, long long leng
                              (uintptr_t)x_dev | (uintptr_t)dy_dev | (uintptr_t)dx_dev, v);
   if (s.samples * s.slabs * s.chunks >= (1LL << 31)) return nsa_fail(NSA_E_ARG, "%s: too many samples", what);
   const GnParams q = {weight_dev, bias_dev, f32};
+  GnTile tile;
+  const bool chunked = gn_tile_threads(samples, length, channels, groups, v, true, tile) == 0;
   float2* ab = (float2*)workspace_dev;
-  float2* part = ab + samples * groups;
+  float2* part = ab + (chunked ? samples * groups : 0);
   if (dtype == NSA_DT_F32) { GN_WIDTHS(float, gn_backward, s, x_dev, dy_dev, q, activation, mean_dev, rstd_dev, dx_dev, dweight_dev, dbias_dev, part, ab, st) }
   else if (dtype == NSA_DT_BF16) { GN_WIDTHS(nsa_bf16, gn_backward, s, x_dev, dy_dev, q, activation, mean_dev, rstd_dev, dx_dev, dweight_dev, dbias_dev, part, ab, st) }
   else { GN_WIDTHS(nsa_f16, gn_backward, s, x_dev, dy_dev, q, activation, mean_dev, rstd_dev, dx_dev, dweight_dev, dbias_dev, part, ab, st) }

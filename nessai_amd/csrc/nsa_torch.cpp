@@ -233,8 +233,8 @@ Tensor embedding(const Tensor& ids_, const Tensor& weight_, double scale, std::o
                     "embedding: expected a table of shape (V, D), got ", weight_.sizes());
   dtype_code(weight_, "embedding: weight");
   const int64_t vocab = weight_.size(0), most = (1LL << 31) - 1;
-  TORCH_CHECK_VALUE(vocab <= most && weight_.size(1) <= most && ids_.numel() <= most,
-                    "embedding: at most 2**31 - 1 rows, columns and indices");
+  TORCH_CHECK_VALUE(vocab <= most && ids_.numel() <= most && weight_.size(1) <= (1 << 20),
+                    "embedding: at most 2**31 - 1 rows and indices and 2**20 columns");
   int64_t padding = -1;
   if (padding_idx.has_value()) {
     TORCH_CHECK_VALUE(-vocab <= *padding_idx && *padding_idx < vocab, "embedding: padding_idx ", *padding_idx,

@@ -518,3 +518,43 @@ def test_two_captured_graphs_replayed_between_eager_calls():
     graphs[0].replay()
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(fresh, outs[0]))
+
+
+def test_a_leaf_changed_before_its_backward_pass_is_noticed():
+    x, w, b, dy = _group_norm_case((6, 5, 8), 2, torch.float32, torch.float32, "silu")
+    w.requires_grad_(True)
+    y = ops.group_norm_act(x, 2, w, b, activation="silu")
+    with torch.no_grad():
+        w.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, [w], dy)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=["f32", "bf16", "f16"])
+def test_unaligned_tensors(t):
+    """Every tensor begins one element behind a 16-byte border: the accesses narrow, the results stay."""
+    def behind(v):
+        room = torch.empty(v.numel() + 1, dtype=v.dtype, device=DEV)
+        room[1:].copy_(v.reshape(-1))
+        return room[1:].view(v.shape)
+
+    for shape, groups in (((300, 64), 8), ((3, 700, 64), 16), ((2, 3, 40), 5)):
+        x, w, b, dy = _group_norm_case(shape, groups, t, t, "silu")
+        results = []
+        for f in (lambda v: v, behind):
+            leaves = [f(v.detach()).requires_grad_(True) for v in (x, w, b)]
+            y = ops.group_norm_act(leaves[0], groups, leaves[1], leaves[2], activation="silu")
+            results.append([y, *torch.autograd.grad(y, leaves, f(dy))])
+        for p, q in zip(*results):
+            # the same arithmetic in another order: float32 sums of at most 128 + samples additions, then a rounding
+            assert float((p.double() - q.double()).norm()) <= (2 * u(t) + 1e-5) * float(p.double().norm())
+    for rows, width in ((9, 64), (900, 64), (900, 40)):
+        ids = _ids(2000, rows, "uneven", torch.int64)
+        w, dy = randn(rows, width, dtype=t), randn(2000, width, seed=1, dtype=t)
+        results = []
+        for f in (lambda v: v, behind):
+            leaf = f(w).requires_grad_(True)
+            out = ops.embedding(ids, leaf, scale=3.0)
+            results.append([out, *torch.autograd.grad(out, [leaf], f(dy))])
+        assert torch.equal(results[0][0], results[1][0])
+        assert float((results[0][1].double() - results[1][1].double()).norm()) <= (2 * u(t) + 1e-5) * float(results[0][1].double().norm())
