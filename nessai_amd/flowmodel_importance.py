@@ -60,6 +60,8 @@ class ImportanceFlowModel(FlowModel):
         self.device = torch.device(self.training_config.get("device_tag", "cuda"))
         if self.device.type != "cuda":
             raise RuntimeError("nessai_amd needs a ROCm device; there is no CPU fallback")
+        if self.flow_config.get("context_net") is not None:
+            raise NotImplementedError("context_net: the importance sampler's flows have no conditional inputs")
         self.inference_device = self.device
         self.initialised = True
 

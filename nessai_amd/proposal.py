@@ -309,6 +309,8 @@ class FlowProposal:
 
         ``resumed``: called from ``resume`` on an unpickled proposal - the reparameterisations
         (with their fitted constants) and the truncation rules are kept as they were."""
+        if dict(self.flow_config or {}).get("context_net") is not None:
+            raise NotImplementedError("context_net: the proposal's flow has no conditional inputs")
         os.makedirs(self.output, exist_ok=True)
         if not resumed or getattr(self, "_reparam", None) is None:
             config = self.reparameterisations

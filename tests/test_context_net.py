@@ -42,3 +42,16 @@ def test_context_flow_from_a_flow_config():
         flow.log_prob(torch.zeros(2, 3))
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         flow.log_prob(torch.zeros(2, 3), context=torch.zeros(2, 3))
+
+
+def test_proposals_refuse_a_context_net(tmp_path):
+    from nessai_amd.flowmodel_importance import ImportanceFlowModel
+    from nessai_amd.model import RosenbrockModel
+    from nessai_amd.proposal import FlowProposal
+
+    config = dict(ftype="nsf", n_inputs=4, context_net=dict(features=2, continuous=1, hidden_features=8))
+    proposal = FlowProposal(RosenbrockModel(4), poolsize=10, output=str(tmp_path), flow_config=config)
+    with pytest.raises(NotImplementedError, match="context_net"):
+        proposal.initialise()
+    with pytest.raises(NotImplementedError, match="context_net"):
+        ImportanceFlowModel(flow_config=config, output=str(tmp_path)).initialise()
