@@ -8,7 +8,7 @@
 // Three ways, by the size of a sample (gn_rows, gn_tile_threads):
 //   rows of a power of two of channels     one pass, shuffles:    200003 x 128 float32, 32 groups: forward 40 us (205 MB at
 //                                          5.1 TB/s), with the backward pass 106 us (512 MB at 4.8 TB/s); as tiles 60 and 197
-//   up to 8192 values (backward 4096)      one pass through LDS:  1000 x 64 x 128 float32: forward 21 us
+//   up to 8192 values (backward 4096)      one pass through LDS:  1000 x 64 x 128 float32: forward 20 us
 //   longer samples                         statistics, their join, then the values once more: 16 x 4096 x 256 bfloat16
 //                                          (34 MB): 11 + 4 + 19 us, the second reading out of the last-level cache
 // A large copy on this card runs at 5.07 TB/s.
@@ -830,6 +830,9 @@ const long long GN_GROUPS_WANTED = 1024;
 // positions of a chunk at least, per row of threads: below it a workgroup's start costs more than its work
 const long long GN_CHUNK_ROWS = 8;
 
+// ... and at most: the float32 sums of a thread stay this short, whatever the lengths
+const long long GN_CHUNK_MOST = 128;
+
 GnShape gn_shape(long long samples, long long length, int channels, int groups, int bytes, uintptr_t addresses, int& v) {
   GnShape s;
   s.samples = samples;
@@ -859,6 +862,7 @@ GnShape gn_shape(long long samples, long long length, int channels, int groups, 
   const long long per = samples * s.slabs;
   long long chunks = std::max(1LL, (GN_GROUPS_WANTED + per - 1) / per);
   chunks = std::min(chunks, std::max(1LL, length / (s.rows * GN_CHUNK_ROWS)));
+  chunks = std::max(chunks, (length * s.tiles + s.rows * GN_CHUNK_MOST - 1) / (s.rows * GN_CHUNK_MOST));
   s.chunk = (length + chunks - 1) / chunks;
   s.chunks = (int)((length + s.chunk - 1) / s.chunk);
   return s;
@@ -909,7 +913,7 @@ size_t gn_tile_lds(const GnTile& q, int threads, bool backward) {
 }
 
 // Whether the one-pass tiles take these samples, with 256 threads (4096 values) or, forward, 512 (8192); 0: they do not.
-// 1000 samples of 8192 float32 values: 21 us in a tile, 30 in the three passes below; of 16384 bfloat16 values the passes are
+// 1000 samples of 8192 float32 values: 20 us in a tile, 30 in the three passes below; of 16384 bfloat16 values the passes are
 // faster (2000 samples: 58 us against 86 in tiles of that size, of which two fit a compute unit).  Backward, where a tile
 // needs twice the LDS, larger ones do not pay.
 int gn_tile_threads(long long samples, long long length, int channels, int groups, int v, bool backward, GnTile& q) {

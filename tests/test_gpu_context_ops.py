@@ -176,6 +176,7 @@ SHAPES = [
     ((1, 8), 2), ((1000, 64), 8), ((333, 20), 5), ((70, 90), 9), ((3, 1, 4), 4), ((2, 7, 6), 6), ((5, 33, 24), 3),
     ((2, 1001, 90), 9), ((4, 16, 16, 32), 8), ((1, 5000, 7), 1), ((3, 2, 3000), 4), ((2, 3, 2100), 1), ((2, 9, 1040), 65),
     ((1, 20_001, 33), 3), ((17, 130, 256), 32), ((4097, 12), 4), ((2, 300, 512), 1), ((3, 40, 2056), 257),
+    ((3, 4096), 512), ((2, 4100), 4100), ((2, 3, 1300), 26), ((1040, 150, 64), 4), ((2, 700, 5000), 1),
 ]
 ACTS = [None, "relu", "tanh", "silu"]
 
