@@ -61,6 +61,17 @@ __device__ __forceinline__ uint32_t emb_key(const ID* ids, long long i, long lon
   return id >= 0 && id < vocab && id != padding ? (uint32_t)id : (uint32_t)vocab;
 }
 
+// the lanes of the wave that are `here` and have this lane's digit
+__device__ __forceinline__ unsigned long long emb_same(uint32_t digit, bool here) {
+  unsigned long long same = __ballot(here);
+#pragma unroll
+  for (int b = 0; b < 8; ++b) {
+    const unsigned long long set = __ballot((digit >> b) & 1u);
+    same &= (digit >> b) & 1u ? set : ~set;
+  }
+  return same;
+}
+
 // digit counts of every tile: counts[digit][tile]; the first pass reads the ids themselves (keys == nullptr)
 template <typename ID, int ITEMS>
 __global__ void __launch_bounds__(EMB_THREADS) emb_count(int n, const ID* __restrict__ ids, long long vocab,
@@ -164,12 +175,7 @@ __global__ void __launch_bounds__(EMB_THREADS) emb_scatter(int n, const ID* __re
   for (int k = 0; k < ITEMS; ++k) {
     const bool here = base + k * 64 < n;
     const uint32_t digit = (key[k] >> shift) & 255u;
-    unsigned long long same = __ballot(here);
-#pragma unroll
-    for (int b = 0; b < 8; ++b) {
-      const unsigned long long set = __ballot((digit >> b) & 1u);
-      same &= (digit >> b) & 1u ? set : ~set;
-    }
+    const unsigned long long same = emb_same(digit, here);
     const uint32_t rank = __popcll(same & ((1ULL << lane) - 1ULL));
     if (here) {
       const uint32_t to = __hip_atomic_load(&place[wave][digit], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) + rank;
@@ -180,6 +186,98 @@ __global__ void __launch_bounds__(EMB_THREADS) emb_scatter(int n, const ID* __re
     if (here && rank == 0) atomicAdd(&place[wave][digit], (uint32_t)__popcll(same));
     __builtin_amdgcn_wave_barrier();
   }
+}
+
+// A few thousand tokens: every pass of the sort in one workgroup, the pairs in LDS between them, as many passes as the table
+// has digits.  The other workgroups of the launch clear the table meanwhile.  The whole gradient of 4096 tokens into 60000 x 32
+// float32 takes 21 us so, 34 with a launch for each step; 1000 into 1000 x 32 take 20 and 27.
+#define EMB_SHORT_THREADS 1024
+#define EMB_SHORT_ITEMS 4
+#define EMB_SHORT (EMB_SHORT_THREADS * EMB_SHORT_ITEMS)
+template <typename T, typename ID>
+__global__ void __launch_bounds__(EMB_SHORT_THREADS) emb_sort_short(int n, const ID* __restrict__ ids, long long vocab,
+                                                                    long long padding, int passes,
+                                                                    uint32_t* __restrict__ keys_out,
+                                                                    uint32_t* __restrict__ pos_out, long long cells,
+                                                                    T* __restrict__ table, uint32_t* __restrict__ runs) {
+  constexpr int WAVES = EMB_SHORT_THREADS / 64;
+  if (blockIdx.x > 0) {
+    for (long long i = (blockIdx.x - 1LL) * EMB_SHORT_THREADS + threadIdx.x; i < cells; i += (gridDim.x - 1LL) * EMB_SHORT_THREADS)
+      table[i] = (T)0.0f;
+    return;
+  }
+  __shared__ uint32_t place[WAVES][256];
+  __shared__ uint32_t wave_sum[4];
+  __shared__ uint32_t key_at[EMB_SHORT], pos_at[EMB_SHORT];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, base = wave * (64 * EMB_SHORT_ITEMS) + lane;
+  if (threadIdx.x == 0) runs[0] = 0;
+  uint32_t key[EMB_SHORT_ITEMS], from[EMB_SHORT_ITEMS];
+#pragma unroll
+  for (int k = 0; k < EMB_SHORT_ITEMS; ++k) {
+    const int i = base + k * 64;
+    key[k] = i < n ? emb_key(ids, i, vocab, padding) : 0u;
+    from[k] = (uint32_t)i;
+  }
+  for (int p = 0; p < passes; ++p) {
+    const int shift = 8 * p;
+    for (int i = threadIdx.x; i < WAVES * 256; i += EMB_SHORT_THREADS) place[i >> 8][i & 255] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < EMB_SHORT_ITEMS; ++k)
+      if (base + k * 64 < n) atomicAdd(&place[wave][(key[k] >> shift) & 255u], 1u);
+    __syncthreads();
+    // a digit per thread of the first four waves: its total, the totals in front of it, and the waves' places
+    uint32_t total = 0, s = 0;
+    if (threadIdx.x < 256) {
+      for (int w = 0; w < WAVES; ++w) total += place[w][threadIdx.x];
+      s = total;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t t = __shfl_up(s, o);
+        if (lane >= o) s += t;
+      }
+      if (lane == 63) wave_sum[wave] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x < 256) {
+      uint32_t at = s - total;
+      for (int w = 0; w < wave; ++w) at += wave_sum[w];
+      for (int w = 0; w < WAVES; ++w) {
+        const uint32_t c = place[w][threadIdx.x];
+        place[w][threadIdx.x] = at;
+        at += c;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < EMB_SHORT_ITEMS; ++k) {
+      const bool here = base + k * 64 < n;
+      const uint32_t digit = (key[k] >> shift) & 255u;
+      const unsigned long long same = emb_same(digit, here);
+      const uint32_t rank = __popcll(same & ((1ULL << lane) - 1ULL));
+      if (here) {
+        const uint32_t to = __hip_atomic_load(&place[wave][digit], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) + rank;
+        key_at[to] = key[k];
+        pos_at[to] = from[k];
+      }
+      __builtin_amdgcn_wave_barrier();
+      if (here && rank == 0) atomicAdd(&place[wave][digit], (uint32_t)__popcll(same));
+      __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < EMB_SHORT_ITEMS; ++k)
+      if (base + k * 64 < n) {
+        key[k] = key_at[base + k * 64];
+        from[k] = pos_at[base + k * 64];
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < EMB_SHORT_ITEMS; ++k)
+    if (base + k * 64 < n) {
+      keys_out[base + k * 64] = key[k];
+      pos_out[base + k * 64] = from[k];
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -584,10 +682,21 @@ void emb_backward_typed(int n, long long vocab, int width, const void* ids, int 
     return emb_few_launch<T, long long, 1>(f, n, (int)vocab, width, ids, padding, dy, scale, dweight, part, s);
   }
   const long long cells = vocab * width;
-  hipLaunchKernelGGL((emb_zero<T>), dim3((unsigned)std::min((cells + EMB_THREADS - 1) / EMB_THREADS, 8192LL)),
-                     dim3(EMB_THREADS), 0, s, cells, (T*)dweight, n == 0 ? nullptr : w.runs);
-  if (n == 0) return;  // (all rows are zero)
-  const int side = ids_bytes == 4 ? emb_sort<int>(n, vocab, ids, padding, w, s) : emb_sort<long long>(n, vocab, ids, padding, w, s);
+  int side = 0;
+  if (n > 0 && n <= EMB_SHORT) {
+    const dim3 grid((unsigned)(1 + std::min((cells + EMB_SHORT_THREADS - 1) / EMB_SHORT_THREADS, 2048LL)));
+    if (ids_bytes == 4)
+      hipLaunchKernelGGL((emb_sort_short<T, int>), grid, dim3(EMB_SHORT_THREADS), 0, s, n, (const int*)ids, vocab, padding,
+                         emb_passes(vocab), w.keys[0], w.pos[0], cells, (T*)dweight, w.runs);
+    else
+      hipLaunchKernelGGL((emb_sort_short<T, long long>), grid, dim3(EMB_SHORT_THREADS), 0, s, n, (const long long*)ids, vocab,
+                         padding, emb_passes(vocab), w.keys[0], w.pos[0], cells, (T*)dweight, w.runs);
+  } else {
+    hipLaunchKernelGGL((emb_zero<T>), dim3((unsigned)std::min((cells + EMB_THREADS - 1) / EMB_THREADS, 8192LL)),
+                       dim3(EMB_THREADS), 0, s, cells, (T*)dweight, n == 0 ? nullptr : w.runs);
+    if (n == 0) return;  // (all rows are zero)
+    side = ids_bytes == 4 ? emb_sort<int>(n, vocab, ids, padding, w, s) : emb_sort<long long>(n, vocab, ids, padding, w, s);
+  }
   const int v = emb_vector(width, sizeof(T), (uintptr_t)dy | (uintptr_t)dweight);
   if constexpr (sizeof(T) == 2) {
     if (v == 8) return emb_reduce_launch<T, 8>(n, vocab, width, w, side, dy, scale, dweight, s);
