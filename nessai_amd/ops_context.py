@@ -47,7 +47,8 @@ def embedding(indices, weight, scale=1.0, padding_idx=None):
 
     The gradient of ``weight`` is dense; its rows are float32 sums over the tokens in a fixed order (equal inputs give equal
     bits), rounded once.  Row ``padding_idx`` gets none.  An index outside ``[0, V)`` cannot be seen without waiting for
-    the device: its row of the result is NaN, and it takes no part in the gradient.  Differentiable once.
+    the device: its row of the result is NaN, and it takes no part in the gradient.  Differentiable once.  At most
+    ``2**31 - 1`` rows and indices and ``2**20`` columns.
     """
     lib.load_torch()
     return torch.ops.nessai_amd.embedding(indices, weight, scale, padding_idx)
