@@ -559,3 +559,50 @@ def test_unaligned_tensors(t):
             results.append([out, *torch.autograd.grad(out, [leaf], f(dy))])
         assert torch.equal(results[0][0], results[1][0])
         assert float((results[0][1].double() - results[1][1].double()).norm()) <= (2 * u(t) + 1e-5) * float(results[0][1].double().norm())
+
+
+# ---- offsets beyond 32 bits -------------------------------------------------------------------------------------------
+
+
+def test_norm_and_clip_of_a_tensor_of_more_than_two_to_the_31_elements():
+    n = 2**31 + 1001  # (4.3 GB; longer than one launch's share of elements)
+    p = torch.nn.Parameter(torch.empty(n, dtype=torch.bfloat16, device=DEV))
+    p.grad = torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    places = [0, 5, 2**31 - 1, 2**31, n - 1]
+    p.grad[places] = 2.0
+    assert abs(float(ops.grad_norm(p.grad)) - math.sqrt(20.0)) <= 2 * U32 * math.sqrt(20.0)
+    ops.clip_grad_norm_([p], 1.0)
+    want = torch.tensor(2.0 / (math.sqrt(20.0) + 1e-6)).bfloat16()
+    assert bool((p.grad[places].cpu() == want).all()) and int(torch.count_nonzero(p.grad)) == len(places)
+
+
+def test_embedding_in_a_table_of_more_than_two_to_the_31_elements():
+    rows, width = 2_200_000, 1024  # (4.5 GB)
+    w = torch.zeros(rows, width, dtype=torch.bfloat16, device=DEV)
+    ids = torch.tensor([rows - 1, 0, 2_097_152, rows - 1, 7] * 30, device=DEV)
+    w[ids.unique()] = randn(4, width).bfloat16()
+    w.requires_grad_(True)
+    out = ops.embedding(ids, w)
+    assert torch.equal(out.detach(), w.detach()[ids])
+    dy = randn(len(ids), width, seed=1, dtype=torch.bfloat16)
+    (dw,) = torch.autograd.grad(out, [w], dy)
+    for row in (rows - 1, 0, 2_097_152, 7):
+        ref = dy.double()[ids == row].sum(0)
+        mag = dy.double()[ids == row].abs().sum(0)
+        assert bool(((dw[row].double() - ref).abs() <= u(torch.bfloat16) * ref.abs() + 100 * U32 * mag).all())  # (60 terms)
+    assert int(torch.count_nonzero(dw.abs().amax(1))) == 4
+
+
+@pytest.mark.parametrize("shape", [(3, 1_500_001, 512), (36_000_000, 64)], ids=["long", "rows"])
+def test_group_norm_of_more_than_two_to_the_31_elements(shape):
+    """The last sample (or rows) agrees with itself alone: other chunks, the same sums to 128 u per chain, then a rounding."""
+    x = torch.empty(shape, dtype=torch.bfloat16, device=DEV).normal_(generator=torch.Generator(device=DEV).manual_seed(1))
+    y = ops.group_norm_act(x, 8, activation="silu")
+    tail = slice(-1, None) if len(shape) == 3 else slice(-1000, None)
+    alone = ops.group_norm_act(x[tail].clone(), 8, activation="silu")
+    assert float((y[tail].double() - alone.double()).norm()) <= (2 * u(torch.bfloat16) + 128 * U32) * float(alone.double().norm())
+    leaf = x.requires_grad_(True)
+    (dx,) = torch.autograd.grad(ops.group_norm_act(leaf, 8, activation="silu"), [leaf], y)
+    end = x.detach()[tail].clone().requires_grad_(True)
+    (want,) = torch.autograd.grad(ops.group_norm_act(end, 8, activation="silu"), [end], y[tail].clone())
+    assert float((dx[tail].double() - want.double()).norm()) <= (2 * u(torch.bfloat16) + 1e-4) * float(want.double().norm())
