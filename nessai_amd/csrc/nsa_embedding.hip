@@ -51,6 +51,25 @@ __global__ void __launch_bounds__(EMB_THREADS) emb_lookup(long long tokens, long
 }
 
 // ---------------------------------------------------------------------------
+// clearing the gradient's rows
+// ---------------------------------------------------------------------------
+
+// `halves` 16-bit words of the table set to zero by `threads` threads of which this is the i-th
+__device__ __forceinline__ void emb_clear(uint16_t* __restrict__ table, long long halves, long long i, long long threads) {
+  if ((uintptr_t)table % 16 == 0 && halves % 8 == 0) {
+    const NsaPack<uint32_t, 4> zero = {{0u, 0u, 0u, 0u}};
+    for (; i < halves / 8; i += threads) reinterpret_cast<NsaPack<uint32_t, 4>*>(table)[i] = zero;
+  } else {
+    for (; i < halves; i += threads) table[i] = 0;
+  }
+}
+
+// the table alone: no tokens
+__global__ void __launch_bounds__(EMB_THREADS) emb_zero(uint16_t* __restrict__ table, long long halves) {
+  emb_clear(table, halves, (long long)blockIdx.x * EMB_THREADS + threadIdx.x, (long long)gridDim.x * EMB_THREADS);
+}
+
+// ---------------------------------------------------------------------------
 // stable radix sort of (id, position)
 // ---------------------------------------------------------------------------
 
@@ -72,12 +91,21 @@ __device__ __forceinline__ unsigned long long emb_same(uint32_t digit, bool here
   return same;
 }
 
-// digit counts of every tile: counts[digit][tile]; the first pass reads the ids themselves (keys == nullptr)
+// digit counts of every tile: counts[digit][tile]; the first pass reads the ids themselves (keys == nullptr), and workgroups
+// of it behind the tiles clear the table and the list of runs
 template <typename ID, int ITEMS>
 __global__ void __launch_bounds__(EMB_THREADS) emb_count(int n, const ID* __restrict__ ids, long long vocab,
                                                          long long padding, const uint32_t* __restrict__ keys, int shift,
-                                                         uint32_t* __restrict__ counts) {
+                                                         int tiles, uint32_t* __restrict__ counts,
+                                                         uint16_t* __restrict__ table, long long halves,
+                                                         uint32_t* __restrict__ runs) {
   __shared__ uint32_t bins[256];
+  if ((int)blockIdx.x >= tiles) {
+    if ((int)blockIdx.x == tiles && threadIdx.x == 0) runs[0] = 0;
+    emb_clear(table, halves, (long long)(blockIdx.x - tiles) * EMB_THREADS + threadIdx.x,
+              (long long)(gridDim.x - tiles) * EMB_THREADS);
+    return;
+  }
   bins[threadIdx.x] = 0;
   __syncthreads();
   const long long base = (long long)blockIdx.x * (EMB_THREADS * ITEMS);
@@ -90,7 +118,7 @@ __global__ void __launch_bounds__(EMB_THREADS) emb_count(int n, const ID* __rest
     }
   }
   __syncthreads();
-  counts[(long long)threadIdx.x * gridDim.x + blockIdx.x] = bins[threadIdx.x];
+  counts[(long long)threadIdx.x * tiles + blockIdx.x] = bins[threadIdx.x];
 }
 
 // one workgroup per digit: its tiles' counts become the counts in front of them, totals[digit] their sum
@@ -194,16 +222,16 @@ __global__ void __launch_bounds__(EMB_THREADS) emb_scatter(int n, const ID* __re
 #define EMB_SHORT_THREADS 1024
 #define EMB_SHORT_ITEMS 4
 #define EMB_SHORT (EMB_SHORT_THREADS * EMB_SHORT_ITEMS)
-template <typename T, typename ID>
+template <typename ID>
 __global__ void __launch_bounds__(EMB_SHORT_THREADS) emb_sort_short(int n, const ID* __restrict__ ids, long long vocab,
                                                                     long long padding, int passes,
                                                                     uint32_t* __restrict__ keys_out,
-                                                                    uint32_t* __restrict__ pos_out, long long cells,
-                                                                    T* __restrict__ table, uint32_t* __restrict__ runs) {
+                                                                    uint32_t* __restrict__ pos_out,
+                                                                    uint16_t* __restrict__ table, long long halves,
+                                                                    uint32_t* __restrict__ runs) {
   constexpr int WAVES = EMB_SHORT_THREADS / 64;
   if (blockIdx.x > 0) {
-    for (long long i = (blockIdx.x - 1LL) * EMB_SHORT_THREADS + threadIdx.x; i < cells; i += (gridDim.x - 1LL) * EMB_SHORT_THREADS)
-      table[i] = (T)0.0f;
+    emb_clear(table, halves, (blockIdx.x - 1LL) * EMB_SHORT_THREADS + threadIdx.x, (gridDim.x - 1LL) * EMB_SHORT_THREADS);
     return;
   }
   __shared__ uint32_t place[WAVES][256];
@@ -283,14 +311,6 @@ __global__ void __launch_bounds__(EMB_SHORT_THREADS) emb_sort_short(int n, const
 // ---------------------------------------------------------------------------
 // sums over equal ids
 // ---------------------------------------------------------------------------
-
-// every row of the table, and the length of the list of runs
-template <typename T>
-__global__ void __launch_bounds__(EMB_THREADS) emb_zero(long long n, T* __restrict__ p, uint32_t* __restrict__ runs) {
-  if (blockIdx.x == 0 && threadIdx.x == 0 && runs != nullptr) runs[0] = 0;
-  for (long long i = (long long)blockIdx.x * EMB_THREADS + threadIdx.x; i < n; i += (long long)gridDim.x * EMB_THREADS)
-    p[i] = (T)0.0f;
-}
 
 // A team of `lanes` lanes takes a chunk of sorted positions, V columns to a lane; EMB_AHEAD rows are asked for before the first
 // is added.  slots[chunk][0]: the partial sum of an id that began in an earlier chunk; [1]: of one that began here and
@@ -644,15 +664,21 @@ void emb_few_launch(const EmbFew& f, long long n, int vocab, int width, const vo
                      f.blocks, part, scale, (T*)dweight);
 }
 
+struct EmbTable {  // the gradient's rows, to be cleared
+  uint16_t* at;
+  long long halves;
+};
+
 template <typename ID, int ITEMS>
-int emb_sort(int n, long long vocab, const ID* ids, long long padding, const EmbSpace& w, hipStream_t s) {
+int emb_sort(int n, long long vocab, const ID* ids, long long padding, const EmbSpace& w, const EmbTable& t, hipStream_t s) {
   const unsigned tiles = (unsigned)emb_tiles(n);
+  const unsigned clear = (unsigned)std::max(1LL, std::min(t.halves / (8 * EMB_THREADS), 4096LL));
   const int passes = emb_passes(vocab);
   for (int p = 0; p < passes; ++p) {
     const uint32_t* keys = p == 0 ? nullptr : w.keys[p & 1];
     const uint32_t* pos = p == 0 ? nullptr : w.pos[p & 1];
-    hipLaunchKernelGGL((emb_count<ID, ITEMS>), dim3(tiles), dim3(EMB_THREADS), 0, s, n, ids, vocab, padding, keys, 8 * p,
-                       w.counts);
+    hipLaunchKernelGGL((emb_count<ID, ITEMS>), dim3(p == 0 ? tiles + clear : tiles), dim3(EMB_THREADS), 0, s, n, ids, vocab,
+                       padding, keys, 8 * p, (int)tiles, w.counts, t.at, t.halves, w.runs);
     hipLaunchKernelGGL(emb_scan, dim3(256), dim3(EMB_THREADS), 0, s, (int)tiles, w.counts, w.totals);
     hipLaunchKernelGGL((emb_scatter<ID, ITEMS>), dim3(tiles), dim3(EMB_THREADS), 0, s, n, ids, vocab, padding, keys, pos,
                        8 * p, w.counts, w.totals, w.keys[(p + 1) & 1], w.pos[(p + 1) & 1]);
@@ -661,9 +687,16 @@ int emb_sort(int n, long long vocab, const ID* ids, long long padding, const Emb
 }
 
 template <typename ID>
-int emb_sort(int n, long long vocab, const void* ids, long long padding, const EmbSpace& w, hipStream_t s) {
-  return n < EMB_MANY ? emb_sort<ID, 4>(n, vocab, (const ID*)ids, padding, w, s)
-                      : emb_sort<ID, 16>(n, vocab, (const ID*)ids, padding, w, s);
+int emb_sort(int n, long long vocab, const void* ids, long long padding, const EmbSpace& w, const EmbTable& t,
+             hipStream_t s) {
+  if (n <= EMB_SHORT) {
+    const long long clear = std::max(1LL, std::min(t.halves / (8 * EMB_SHORT_THREADS), 2048LL));
+    hipLaunchKernelGGL((emb_sort_short<ID>), dim3((unsigned)(1 + clear)), dim3(EMB_SHORT_THREADS), 0, s, n, (const ID*)ids,
+                       vocab, padding, emb_passes(vocab), w.keys[0], w.pos[0], t.at, t.halves, w.runs);
+    return 0;
+  }
+  return n < EMB_MANY ? emb_sort<ID, 4>(n, vocab, (const ID*)ids, padding, w, t, s)
+                      : emb_sort<ID, 16>(n, vocab, (const ID*)ids, padding, w, t, s);
 }
 
 template <typename T>
@@ -681,22 +714,14 @@ void emb_backward_typed(int n, long long vocab, int width, const void* ids, int 
       if (f.words == 2) return emb_few_launch<T, long long, 2>(f, n, (int)vocab, width, ids, padding, dy, scale, dweight, part, s);
     return emb_few_launch<T, long long, 1>(f, n, (int)vocab, width, ids, padding, dy, scale, dweight, part, s);
   }
-  const long long cells = vocab * width;
-  int side = 0;
-  if (n > 0 && n <= EMB_SHORT) {
-    const dim3 grid((unsigned)(1 + std::min((cells + EMB_SHORT_THREADS - 1) / EMB_SHORT_THREADS, 2048LL)));
-    if (ids_bytes == 4)
-      hipLaunchKernelGGL((emb_sort_short<T, int>), grid, dim3(EMB_SHORT_THREADS), 0, s, n, (const int*)ids, vocab, padding,
-                         emb_passes(vocab), w.keys[0], w.pos[0], cells, (T*)dweight, w.runs);
-    else
-      hipLaunchKernelGGL((emb_sort_short<T, long long>), grid, dim3(EMB_SHORT_THREADS), 0, s, n, (const long long*)ids, vocab,
-                         padding, emb_passes(vocab), w.keys[0], w.pos[0], cells, (T*)dweight, w.runs);
-  } else {
-    hipLaunchKernelGGL((emb_zero<T>), dim3((unsigned)std::min((cells + EMB_THREADS - 1) / EMB_THREADS, 8192LL)),
-                       dim3(EMB_THREADS), 0, s, cells, (T*)dweight, n == 0 ? nullptr : w.runs);
-    if (n == 0) return;  // (all rows are zero)
-    side = ids_bytes == 4 ? emb_sort<int>(n, vocab, ids, padding, w, s) : emb_sort<long long>(n, vocab, ids, padding, w, s);
+  const EmbTable t = {(uint16_t*)dweight, vocab * width * (long long)(sizeof(T) / 2)};
+  if (n == 0) {  // (all rows are zero)
+    hipLaunchKernelGGL(emb_zero, dim3((unsigned)std::max(1LL, std::min(t.halves / (8 * EMB_THREADS), 4096LL))),
+                       dim3(EMB_THREADS), 0, s, t.at, t.halves);
+    return;
   }
+  const int side = ids_bytes == 4 ? emb_sort<int>(n, vocab, ids, padding, w, t, s)
+                                  : emb_sort<long long>(n, vocab, ids, padding, w, t, s);
   const int v = emb_vector(width, sizeof(T), (uintptr_t)dy | (uintptr_t)dweight);
   if constexpr (sizeof(T) == 2) {
     if (v == 8) return emb_reduce_launch<T, 8>(n, vocab, width, w, side, dy, scale, dweight, s);
