@@ -10,15 +10,15 @@
 // table's size has digits - and the sums then run over neighbours, in the order of the positions: equal inputs give equal
 // bits.  The sorted list is cut into chunks of equal length, whatever the frequencies of the ids: an id inside one chunk
 // is finished there; one that runs over a chunk's border leaves float32 partial sums, which a second kernel joins.
-// 131072 rows of 320 bfloat16 into 32768 (84 MB in, 21 MB out): clearing 6, sorting 2 x 11, adding 21, joining 13 us.  The sort
-// is bound by the latency of its short kernels, the sums by gathering rows (4.0 TB/s).
+// 131072 rows of 320 bfloat16 into 32768 (84 MB in, 21 MB out): 61 us; sorting and clearing 2 x 12, adding 21, joining 13.  The
+// sort is bound by the latency of its short kernels, the sums by gathering rows (4.0 TB/s).
 #include <hip/hip_runtime.h>
 #include <algorithm>
 
 #include "nsa_elem.h"
 
 #define EMB_THREADS 256
-#define EMB_MANY 400000                       // tokens from which a sorting tile has 16 keys per thread instead of 4
+#define EMB_MANY 1500000                      // tokens from which a sorting tile has 16 keys per thread instead of 4
 #define EMB_AHEAD 8                           // rows in flight per team
 #define EMB_FEW_AHEAD 16                      // the same where a row is four bytes a lane
 #define EMB_FEW 64                            // (rows + 1) x columns per lane of a gradient summed in LDS (64 KB)
@@ -529,15 +529,16 @@ int emb_passes(long long vocab) {  // 8 bits each; the largest key is `vocab` it
   return (bits + 7) / 8;
 }
 
-// Sorting tiles.  A few hundred thousand tokens in tiles of 4096 would leave most compute units idle: 131072 tokens, a pass of
-// 22 us in 32 tiles.
+// Sorting tiles of 1024 or 4096 keys: the larger ones need fewer counts, the smaller ones leave no compute unit idle.  The whole
+// gradient into 5000 x 8 float32 with 4 and with 16 keys per thread: 100000 tokens 43 and 58 us, 600000 82 and 90, 10^6 97 and
+// 100, 4 x 10^6 280 and 255.
 long long emb_tiles(long long n) {
   const int tile = EMB_THREADS * (n < EMB_MANY ? 4 : 16);
   return (n + tile - 1) / tile;
 }
 
-// sorted positions per team of the reduction: short chunks for few tokens (all compute units at work), longer ones for many
-// (fewer partial sums to join)
+// sorted positions per team of the reduction: short chunks for few tokens (all compute units at work; 20000 x 64 float32: 34 us in
+// chunks of 32, 41 of 64), longer ones for many (fewer partial sums to join)
 int emb_chunk(long long n) {
   int len = 32;
   while (len < 256 && n / len > 16384) len *= 2;
