@@ -511,16 +511,18 @@ __device__ __forceinline__ float gn_team_sum(float a, int team) {
   return a;
 }
 
-// group, weight and bias of the V channels at value e of a tile
-template <typename T, int V>
-__device__ __forceinline__ void gn_channels(const GnTile& q, const GnParams& par, int e, int (&g)[V], float (&w)[V],
+// group, weight and bias of the V channels at value e of a tile; wb: {weight, bias} of every channel, in LDS (from memory they
+// cost a load per value where a thread's channels change from access to access)
+template <int V>
+__device__ __forceinline__ void gn_channels(const GnTile& q, const float2* wb, int e, int (&g)[V], float (&w)[V],
                                             float (&b)[V]) {
   const int c = e - gn_div(e, q.by_channels) * q.channels;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
+    const float2 t = wb[c + i];
     g[i] = gn_div(c + i, q.by_cpg);
-    w[i] = gn_param<T>(par.w, par.f32, c + i, 1.0f);
-    b[i] = gn_param<T>(par.b, par.f32, c + i, 0.0f);
+    w[i] = t.x;
+    b[i] = t.y;
   }
 }
 
@@ -532,6 +534,9 @@ __global__ void __launch_bounds__(THREADS) gn_tile_forward(GnTile q, const T* __
   extern __shared__ float lds[];
   float* buf = lds;                                    // [THREADS * GN_EACH]
   float2* stat = (float2*)(lds + THREADS * GN_EACH);   // [per * groups]
+  float2* wb = stat + q.per * q.groups;                // [channels]
+  for (int c = threadIdx.x; c < q.channels; c += THREADS)
+    wb[c] = make_float2(gn_param<T>(par.w, par.f32, c, 1.0f), gn_param<T>(par.b, par.f32, c, 0.0f));
   const long long first = (long long)blockIdx.x * q.per;
   const int here = q.samples - first < q.per ? (int)(q.samples - first) : q.per;
   const int values = here * q.values;
@@ -576,7 +581,7 @@ __global__ void __launch_bounds__(THREADS) gn_tile_forward(GnTile q, const T* __
     const int e = (k * THREADS + threadIdx.x) * V;
     if (e >= values) continue;
     const int s = gn_div(e, q.by_values);
-    if (k == 0 || !q.fixed) gn_channels<T, V>(q, par, e, g, w, b);
+    if (k == 0 || !q.fixed) gn_channels<V>(q, wb, e, g, w, b);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float2 t = stat[s * q.groups + g[i]];
@@ -599,14 +604,15 @@ __global__ void __launch_bounds__(THREADS) gn_tile_backward(GnTile q, const T* _
   float* bz = lds;                                            // [THREADS * GN_EACH]  dz
   float* bzx = lds + THREADS * GN_EACH;                       //                      dz xh
   float2* ab = (float2*)(lds + 2 * THREADS * GN_EACH);        // [per * groups]
-  float* bw = (float*)(ab + q.per * q.groups);                // [channels] weights
-  float2* cols = (float2*)(bw + (q.channels + 1) / 2 * 2);    // [subs][channels]
+  float2* stat = ab + q.per * q.groups;                       // [per * groups]
+  float2* wb = stat + q.per * q.groups;                       // [channels] weight, bias
+  float2* cols = wb + q.channels;                             // [subs][channels]
   const int subs = q.channels < THREADS ? THREADS / q.channels : 1;
-  for (int c = threadIdx.x; c < q.channels; c += THREADS) bw[c] = gn_param<T>(par.w, par.f32, c, 1.0f);
+  for (int c = threadIdx.x; c < q.channels; c += THREADS)
+    wb[c] = make_float2(gn_param<T>(par.w, par.f32, c, 1.0f), gn_param<T>(par.b, par.f32, c, 0.0f));
   for (int i = threadIdx.x; i < subs * q.channels; i += THREADS) cols[i] = make_float2(0.0f, 0.0f);
   const float m = (float)q.length * (float)q.cpg;
   const long long tiles = (q.samples + q.per - 1) / q.per;
-  __syncthreads();
   for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const long long first = tile * q.per, base = first * q.values;
     const int here = q.samples - first < q.per ? (int)(q.samples - first) : q.per;
@@ -621,16 +627,20 @@ __global__ void __launch_bounds__(THREADS) gn_tile_backward(GnTile q, const T* _
         nsa_load<T, V>(dy + base + e, z[k]);
       }
     }
+    for (int p = threadIdx.x; p < here * q.groups; p += THREADS)
+      stat[p] = make_float2(mean[first * q.groups + p], rstd[first * q.groups + p]);
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < STEPS; ++k) {
       const int e = (k * THREADS + threadIdx.x) * V;
       if (e >= values) continue;
-      const long long p = (first + gn_div(e, q.by_values)) * q.groups;
-      if (k == 0 || !q.fixed) gn_channels<T, V>(q, par, e, g, w, b);
+      const int p = gn_div(e, q.by_values) * q.groups;
+      if (k == 0 || !q.fixed) gn_channels<V>(q, wb, e, g, w, b);
       float zx[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        v[k][i] = (v[k][i] - mean[p + g[i]]) * rstd[p + g[i]];
+        const float2 t = stat[p + g[i]];
+        v[k][i] = (v[k][i] - t.x) * t.y;
         z[k][i] *= gn_slope<ACT>(fmaf(v[k][i], w[i], b[i]));
         zx[i] = z[k][i] * v[k][i];
       }
@@ -644,8 +654,8 @@ __global__ void __launch_bounds__(THREADS) gn_tile_backward(GnTile q, const T* _
         const int s = p / q.groups, g = p - s * q.groups;
         float a = 0.0f, b = 0.0f;
         gn_walk(q, s, g, lane, [&](int at, int c) {
-          a = fmaf(bw[c], bz[at], a);
-          b = fmaf(bw[c], bzx[at], b);
+          a = fmaf(wb[c].x, bz[at], a);
+          b = fmaf(wb[c].x, bzx[at], b);
         });
         a = gn_team_sum(a, q.team);
         b = gn_team_sum(b, q.team);
@@ -671,18 +681,17 @@ __global__ void __launch_bounds__(THREADS) gn_tile_backward(GnTile q, const T* _
         const int e = (k * THREADS + threadIdx.x) * V;
         if (e >= values) continue;
         const int s = gn_div(e, q.by_values);
-        if (!q.fixed) gn_channels<T, V>(q, par, e, g, w, b);
+        if (!q.fixed) gn_channels<V>(q, wb, e, g, w, b);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const float2 t = ab[s * q.groups + g[i]];
-          z[k][i] = rstd[(first + s) * q.groups + g[i]] * (w[i] * z[k][i] - t.x - v[k][i] * t.y);
+          z[k][i] = stat[s * q.groups + g[i]].y * (w[i] * z[k][i] - t.x - v[k][i] * t.y);
         }
         nsa_store<T, V>(dx + base + e, z[k]);
       }
     }
-    // (the next tile's dz is written to LDS by threads that have passed the barrier above: nothing reads the old one)
+    __syncthreads();  // (the next tile's statistics take the place of these)
   }
-  __syncthreads();
   if (part != nullptr)
     for (int c = threadIdx.x; c < q.channels; c += THREADS) {
       float2 t = cols[c];
@@ -906,10 +915,9 @@ bool gn_rows(const GnShape& s, int v, GnRows& q) {
 }
 
 size_t gn_tile_lds(const GnTile& q, int threads, bool backward) {
-  const size_t stat = (size_t)q.per * q.groups * sizeof(float2);
-  if (!backward) return (size_t)threads * GN_EACH * 4 + stat;
-  return (size_t)threads * GN_EACH * 8 + stat + (size_t)(q.channels + 1) / 2 * 8 +
-         (size_t)std::max(threads, q.channels) * sizeof(float2);
+  const size_t stat = (size_t)q.per * q.groups * sizeof(float2), wb = (size_t)q.channels * sizeof(float2);
+  if (!backward) return (size_t)threads * GN_EACH * 4 + stat + wb;
+  return (size_t)threads * GN_EACH * 8 + 2 * stat + wb + (size_t)std::max(threads, q.channels) * sizeof(float2);
 }
 
 // Whether the one-pass tiles take these samples, with 256 threads (4096 values) or, forward, 512 (8192); 0: they do not.

@@ -47,6 +47,7 @@ GRADS = {
     "minibatch_flow": [(16, 64), (64,), (64, 64), (64,), (368, 64), (368,)] * 3,
     "empty_among_them": [(0,), (5,), (0, 4), (7, 1)],
     "many": [(1 + 37 * i % 211,) for i in range(701)],       # several launches
+    "tiny": [(1 + 7 * i % 23,) for i in range(577)],
     "large": [(1_000_003,), (3,), (70_001, 5), (1,)],
 }
 
@@ -358,6 +359,7 @@ TABLES = [
     (4096, 255, 64, "uniform"), (4097, 256, 33, "uneven"), (9001, 257, 320, "uneven"), (30_000, 65_536, 24, "uneven"),
     (20_000, 40, 100, "one"), (333, 9, 1030, "uniform"), (100_000, 5000, 7, "uneven"), (2048, 100_000, 128, "uniform"),
     (300, 17, 2050, "uneven"), (50_000, 3, 3, "sorted"), (12_345, 700, 48, "sorted"),
+    (1_600_003, 3000, 4, "uniform"),
 ]
 
 
