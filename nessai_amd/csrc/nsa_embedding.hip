@@ -509,16 +509,14 @@ int emb_vector(int width, int bytes, uintptr_t addresses) {
   return v;
 }
 
-// Lanes of a team, a power of two.  A short row: one access of each lane.  A longer one: eight lanes or more (128 bytes side
-// by side), as many as leave at most an eighth of them idle in its last round; 40 accesses, for one, are five rounds of 8.
-int emb_lanes(int vectors) {
+// Lanes of a team, a power of two, for rows of `vectors` accesses of `bytes` each.  A short row: one access of each lane.  A
+// longer one: as many lanes as make 128 bytes side by side (a wave at most), or more where that leaves at most an eighth of
+// them idle in their last round; 40 accesses of 16 bytes, for one, are five rounds of 8.
+int emb_lanes(int vectors, int bytes) {
+  const int least = std::min(64, 128 / bytes);
   int best = 1;
-  if (vectors <= 8) {
-    while (best < vectors) best *= 2;
-    return best;
-  }
-  best = 8;
-  for (int l = 16; l <= 64; l *= 2)
+  while (best < least && best < vectors) best *= 2;
+  for (int l = 2 * best; l <= 64 && vectors > best; l *= 2)
     if ((vectors + l - 1) / l * l * 8 <= vectors * 9) best = l;
   return best;
 }
@@ -617,7 +615,7 @@ int emb_done(const char* what) {
 template <typename T, typename ID, int V>
 void emb_lookup_launch(long long tokens, long long vocab, int width, const void* ids, const void* weight, float scale,
                        void* out, hipStream_t s) {
-  const int lanes = emb_lanes((width + V - 1) / V), teams = EMB_THREADS / lanes;
+  const int lanes = emb_lanes((width + V - 1) / V, V * (int)sizeof(T)), teams = EMB_THREADS / lanes;
   const long long groups = (tokens + teams - 1) / teams;
   hipLaunchKernelGGL((emb_lookup<T, ID, V>), dim3((unsigned)std::min(groups, 65536LL)), dim3(EMB_THREADS), 0, s, tokens,
                      vocab, width, (const ID*)ids, (const T*)weight, scale, lanes, (T*)out);
@@ -638,7 +636,7 @@ void emb_lookup_typed(long long tokens, long long vocab, int width, const void* 
 template <typename T, int V>
 void emb_reduce_launch(int n, long long vocab, int width, const EmbSpace& w, int side, const void* dy, float scale,
                        void* dweight, hipStream_t s) {
-  const int lanes = emb_lanes((width + V - 1) / V), teams = EMB_THREADS / lanes, len = emb_chunk(n);
+  const int lanes = emb_lanes((width + V - 1) / V, V * (int)sizeof(T)), teams = EMB_THREADS / lanes, len = emb_chunk(n);
   const long long chunks = ((long long)n + len - 1) / len;
   const int slabs = (width + lanes * V - 1) / (lanes * V);
   hipLaunchKernelGGL((emb_reduce<T, V>), dim3((unsigned)((chunks + teams - 1) / teams), slabs), dim3(EMB_THREADS), 0, s, n,
