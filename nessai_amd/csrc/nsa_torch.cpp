@@ -13,6 +13,7 @@
 
 #include <cmath>
 #include <optional>
+#include <utility>
 #include <vector>
 
 #include "../../include/nessai_amd.h"
@@ -76,6 +77,12 @@ bool wants_grad(std::initializer_list<const Tensor*> tensors) {
   for (const Tensor* t : tensors)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+
+// A tangent (forward-mode differentiation) would be lost: results are allocated here, outside torch's own derivatives.
+void no_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), what,
+              " has no forward-mode derivative: it was given a tensor with a tangent (torch.autograd.forward_ad, torch.func.jvp)");
 }
 
 void once(const char* what) {
@@ -161,6 +168,7 @@ Tensor group_norm_act(const Tensor& x_, int64_t groups, const std::optional<Tens
                     " channels cannot be divided into ", groups, " groups");
   TORCH_CHECK_VALUE(eps >= 0.0, "eps must not be negative (got ", eps, ")");
   Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
+  for (const Tensor* t : {&x_, &std::as_const(weight), &std::as_const(bias)}) no_tangent(*t, "group_norm_act");
   const char* names[] = {"weight", "bias"};
   Tensor* params[] = {&weight, &bias};
   for (int i = 0; i < 2; ++i) {
@@ -232,6 +240,7 @@ Tensor embedding(const Tensor& ids_, const Tensor& weight_, double scale, std::o
   TORCH_CHECK_VALUE(weight_.dim() == 2 && weight_.size(0) >= 1 && weight_.size(1) >= 1,
                     "embedding: expected a table of shape (V, D), got ", weight_.sizes());
   dtype_code(weight_, "embedding: weight");
+  no_tangent(weight_, "embedding");
   const int64_t vocab = weight_.size(0), most = (1LL << 31) - 1;
   TORCH_CHECK_VALUE(vocab <= most && ids_.numel() <= most && weight_.size(1) <= (1 << 20),
                     "embedding: at most 2**31 - 1 rows and indices and 2**20 columns");
@@ -253,6 +262,7 @@ void check_gradients(const std::vector<Tensor>& tensors, const char* what) {
   for (const Tensor& t : tensors) {
     TORCH_CHECK_TYPE(t.layout() == at::kStrided, what, ": gradients must be dense (got ", t.layout(), ")");
     dtype_code(t, what);
+    no_tangent(t, what);
     TORCH_CHECK_VALUE(t.device() == tensors[0].device(), what, ": gradients on several devices: ", tensors[0].device(), ", ", t.device());
   }
   on_device(tensors[0], what);

@@ -12,7 +12,8 @@ that makes it to torch.  What such a net is built from and trained with has kern
 =======================  ===================================================================================
 
 Values are float32, bfloat16 or float16; sums and statistics are held in float32 or wider and results are rounded once.
-There is no CPU implementation; float64 is refused, never cast down.  Every call enqueues on the current stream of the
+There is no CPU implementation; float64 is refused, never cast down.  Derivatives are first-order and reverse-mode: a tensor
+with a tangent (``torch.autograd.forward_ad``, ``torch.func.jvp``) is refused.  Every call enqueues on the current stream of the
 tensors' device, waits for nothing (but ``error_if_nonfinite``) and may be captured into a HIP graph.  The functions here name
 the arguments; ``csrc/nsa_torch.cpp`` checks them, allocates and records for autograd.
 """

@@ -73,6 +73,34 @@ def test_gradient_norm_refuses_what_it_cannot_compute():
         ops.grad_norm(torch.eye(3).to_sparse())
 
 
+def test_tangents_are_refused():
+    """Forward-mode differentiation: the operators have no rule for it, and a result without a tangent reads as a zero."""
+    from torch.autograd import forward_ad as fwd
+
+    def dual(t):
+        return fwd.make_dual(t, torch.ones_like(t))
+
+    x, w, i = torch.randn(4, 12), torch.ones(12), torch.tensor([1, 2])
+    with fwd.dual_level(), torch.no_grad():
+        for call in (
+            lambda: ops.group_norm_act(dual(x), 3),
+            lambda: ops.group_norm_act(x, 3, weight=dual(w)),
+            lambda: ops.group_norm_act(x, 3, bias=dual(w)),
+            lambda: ops.embedding(i, dual(x)),
+            lambda: ops.grad_norm([w, dual(x)]),
+        ):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        p = torch.nn.Parameter(torch.zeros(12))
+        p.grad = dual(w)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.clip_grad_norm_([p], 1.0)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda v: ops.group_norm_act(v, 3), (x,), (torch.ones_like(x),))
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda v: ops.embedding(i, v), (x,), (torch.ones_like(x),))
+
+
 def _norm_args(places, sizes, codes):
     n = len(places)
     return (n, (ctypes.c_void_p * n)(*places), (ctypes.c_longlong * n)(*sizes), (ctypes.c_int * n)(*codes))
