@@ -59,12 +59,27 @@ class GroupNormAct(nn.Module):
         return ops.group_norm_act(x, self.num_groups, self.weight, self.bias, eps=self.eps, activation=self.activation)
 
 
+def exact_labels(dtype):
+    """The numbers of labels, counted from zero, that a floating-point type tells apart (2**24 in float32)."""
+    return int(2.0 / torch.finfo(dtype).eps)
+
+
+def label_indices(labels):
+    """Labels as int64.  What is no whole number of the type's exact range - a fraction, NaN, an infinity - becomes -1, a row
+    that no table has: cast as it is, 0.9 and -0.5 would be label 0, and NaN whatever the device makes of it."""
+    if not labels.is_floating_point():
+        return labels.to(torch.int64)
+    whole = (labels == labels.floor()) & (labels.abs() < exact_labels(labels.dtype))
+    return torch.where(whole, labels, -1.0).to(torch.int64)
+
+
 class ContextNet(nn.Module):
     """``(n, len(labels) + continuous)`` conditional inputs -> the ``(n, features)`` context of a flow.
 
-    The first ``len(labels)`` columns hold labels, whole numbers in ``[0, labels[k])`` (a label outside gives a context of
-    NaN, so that the loss shows it), the others continuous values.  Their embeddings and a linear map are added, then
-    ``num_layers`` times group norm, activation and a linear layer follow.
+    The first ``len(labels)`` columns hold labels, whole numbers in ``[0, labels[k])`` (anything else - a label outside, a
+    fraction, NaN - gives a context of NaN, so that the loss shows it), the others continuous values.  Their embeddings and a
+    linear map are added, then ``num_layers`` times group norm, activation and a linear layer follow.  Inputs of a type in
+    which some labels of a table run together (more than 2**24 in float32) are refused.
     """
 
     def __init__(self, features, labels=(), continuous=0, hidden_features=32, num_layers=2, num_groups=4,
@@ -90,7 +105,9 @@ class ContextNet(nn.Module):
             raise ValueError(f"Expected conditional inputs of shape (N, {columns}), got {tuple(inputs.shape)}")
         parts = []
         if self.labels:
-            ids = inputs[:, : len(self.labels)].to(torch.int64)
+            if inputs.is_floating_point() and max(self.labels) > exact_labels(inputs.dtype):
+                raise ValueError(f"{max(self.labels)} labels cannot be told apart in inputs of type {inputs.dtype}")
+            ids = label_indices(inputs[:, : len(self.labels)])
             parts = [embedding(ids[:, k]) for k, embedding in enumerate(self.embeddings)]
         if self.continuous_layer is not None:
             parts.append(self.continuous_layer(inputs[:, len(self.labels) :].to(torch.float32)))

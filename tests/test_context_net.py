@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from nessai_amd.flows import ContextFlow, ContextNet, Embedding, GroupNormAct, NeuralSplineFlow, RealNVP, configure_model
+from nessai_amd.flows.context import label_indices
 
 
 def test_context_net_checks_its_arguments():
@@ -21,6 +22,31 @@ def test_context_net_checks_its_arguments():
     table = Embedding(5, 4, padding_idx=2)
     assert not table.weight[2].any() and table.weight[[0, 1, 3, 4]].all()
     assert GroupNormAct(2, 4, activation=torch.nn.functional.silu).activation == "silu"
+
+
+def test_labels_that_are_not_whole_numbers_have_no_row():
+    inf = float("inf")
+    values = [0.0, 3.0, -0.5, 0.9, 2.7, 2.0**24 - 1, 2.0**24, 2.0**40, 1e30, inf, -inf, float("nan"), -1.0, -0.0]
+    want = [0, 3, -1, -1, -1, 2**24 - 1, -1, -1, -1, -1, -1, -1, -1, 0]
+    assert label_indices(torch.tensor(values)).tolist() == want
+    assert label_indices(torch.tensor(values, dtype=torch.float64)).tolist()[:8] == want[:6] + [2**24, 2**40]
+    for dtype, most in ((torch.float16, 2**11), (torch.bfloat16, 2**8)):
+        ids = label_indices(torch.tensor([0.0, 2.5, most - 1, most, inf, float("nan")], dtype=dtype))
+        assert ids.dtype == torch.int64 and ids.tolist() == [0, -1, most - 1, -1, -1, -1]
+    assert label_indices(torch.tensor([2**30, -3], dtype=torch.int32)).tolist() == [2**30, -3]
+
+
+def test_inputs_that_cannot_hold_the_labels_are_refused():
+    net = ContextNet(2, labels=[3, 2**24 + 1], hidden_features=4, num_groups=1)
+    with pytest.raises(ValueError, match="told apart"):
+        net(torch.zeros(5, 2))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        net(torch.zeros(5, 2, dtype=torch.int64))
+    net = ContextNet(2, labels=[2**8 + 1], hidden_features=4, num_groups=1)
+    with pytest.raises(ValueError, match="told apart"):
+        net(torch.zeros(5, 1, dtype=torch.bfloat16))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        net(torch.zeros(5, 1, dtype=torch.float16))
 
 
 def test_context_flow_from_a_flow_config():

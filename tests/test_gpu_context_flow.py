@@ -201,6 +201,21 @@ def test_methods_of_a_context_flow_agree():
         both.flow.log_prob(x.clone(), context=both.net(inputs.clone()))
 
 
+def test_labels_that_are_not_whole_numbers_show_in_their_rows():
+    """NaN, fractions and infinities are no labels: their rows are NaN, in evaluation and in the net itself, and no other is."""
+    torch.manual_seed(2)
+    both = ContextFlow(NeuralSplineFlow(4, 16, 2, 2, context_features=3), ContextNet(3, labels=[5], continuous=1))
+    both.to(DEV)
+    both.eval()
+    inputs = _inputs(both.net, 12).to(DEV)
+    bad = [math.nan, -0.5, 2.7, 0.9, math.inf, -math.inf, -1.0, 5.0, 2.0**40]
+    inputs[: len(bad), 0] = torch.tensor(bad, device=DEV)
+    with torch.no_grad():
+        assert both.net(inputs)[: len(bad)].isnan().all() and torch.isfinite(both.net(inputs)[len(bad) :]).all()
+        lp = both.log_prob(torch.randn(12, 4, device=DEV), context=inputs)
+    assert lp[: len(bad)].isnan().all() and torch.isfinite(lp[len(bad) :]).all()
+
+
 @pytest.mark.parametrize("ftype", ["nsf", "realnvp"])
 def test_flow_model_trains_a_context_flow(tmp_path, ftype):
     """``FlowModel.train(conditional=...)`` of a flow with a context net runs, keeps the best weights, saves and reloads."""
