@@ -204,6 +204,8 @@ class FlowModel:
             raise ValueError("Cannot train with non-finite samples!")
         if weights is not None and conditional is not None:
             raise RuntimeError("weights and conditional inputs not supported")
+        if conditional is not None and not np.isfinite(np.asarray(conditional, dtype=np.float64)).all():
+            raise ValueError("Cannot train with non-finite conditional inputs!")
         idx = self.rng.permutation(samples.shape[0])
         samples = samples[idx]
         if conditional is not None:

@@ -81,3 +81,18 @@ def test_proposals_refuse_a_context_net(tmp_path):
         proposal.initialise()
     with pytest.raises(NotImplementedError, match="context_net"):
         ImportanceFlowModel(flow_config=config, output=str(tmp_path)).initialise()
+
+
+def test_training_refuses_conditional_inputs_that_are_not_finite(tmp_path):
+    import numpy as np
+
+    from nessai_amd.flowmodel import FlowModel
+
+    fm = FlowModel(flow_config=dict(ftype="nsf", n_inputs=2, context_features=1), output=str(tmp_path))
+    fm.initialised = True  # (the split is host work: no flow is built for it)
+    x, c = np.zeros((20, 2)), np.zeros(20)
+    for bad in (np.nan, np.inf):
+        c[3] = bad
+        for conditional in (c, c[:, None]):
+            with pytest.raises(ValueError, match="non-finite conditional"):
+                fm.prep_data(x, val_size=0.1, batch_size=5, conditional=conditional)
