@@ -103,6 +103,8 @@ class ContextNet(nn.Module):
         columns = len(self.labels) + self.continuous
         if inputs.dim() != 2 or inputs.shape[1] != columns:
             raise ValueError(f"Expected conditional inputs of shape (N, {columns}), got {tuple(inputs.shape)}")
+        if self.continuous and inputs.dtype == torch.float64:
+            raise TypeError("ContextNet computes in float32 and casts nothing down silently: the conditional inputs are float64")
         parts = []
         if self.labels:
             if inputs.is_floating_point() and max(self.labels) > exact_labels(inputs.dtype):

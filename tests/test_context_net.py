@@ -49,6 +49,14 @@ def test_inputs_that_cannot_hold_the_labels_are_refused():
         net(torch.zeros(5, 1, dtype=torch.float16))
 
 
+def test_float64_columns_are_refused():
+    """As everywhere in the package; labels alone lose nothing by their type."""
+    with pytest.raises(TypeError, match="float64"):
+        ContextNet(2, labels=[3], continuous=1, hidden_features=4)(torch.zeros(5, 2, dtype=torch.float64))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ContextNet(2, labels=[3], hidden_features=4)(torch.zeros(5, 1, dtype=torch.float64))
+
+
 def test_context_flow_from_a_flow_config():
     config = dict(n_inputs=3, n_neurons=8, n_blocks=2, n_layers=1, ftype="nsf",
                   context_net=dict(features=4, labels=[6], continuous=2, hidden_features=8))
