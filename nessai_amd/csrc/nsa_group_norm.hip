@@ -92,15 +92,21 @@ __device__ __forceinline__ float gn_param(const void* p, int f32, int c, float n
   return f32 ? ((const float*)p)[c] : (float)((const T*)p)[c];
 }
 
+// Which workgroup of a launch this is.  A launch holds fewer than 2^32 threads in a dimension - 2^24 workgroups of 256, which
+// many samples of many groups pass - so more than GN_GRID_X workgroups lie in rows of as many (gn_grid); those behind the
+// last one have nothing to do, each as a whole.
+#define GN_GRID_X (1 << 20)
+__device__ __forceinline__ long long gn_block() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }
+
 struct GnPlace {  // what this workgroup works on
-  long long n, l0, l1;
+  long long n, l0, l1;  // n >= samples: nothing
   int slab, chunk, j, r;
   bool active;
 };
 
 __device__ __forceinline__ GnPlace gn_place(const GnShape& s) {
   GnPlace p;
-  long long b = blockIdx.x;
+  long long b = gn_block();
   p.chunk = (int)(b % s.chunks);
   b /= s.chunks;
   p.slab = (int)(b % s.slabs);
@@ -158,6 +164,7 @@ __global__ void __launch_bounds__(GN_THREADS) gn_stats(GnShape s, const T* __res
   __shared__ float means[GN_THREADS * V], devs[GN_THREADS * V];
   __shared__ int counts[GN_THREADS];
   const GnPlace p = gn_place(s);
+  if (p.n >= s.samples) return;
   float shift[V], sum[V], sq[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) shift[i] = sum[i] = sq[i] = 0.0f;
@@ -224,7 +231,7 @@ __global__ void __launch_bounds__(GN_THREADS) gn_stats(GnShape s, const T* __res
 // the chunks of a (sample, group) joined in 64 bits: a wave each, lane by lane, then lane with lane
 __global__ void __launch_bounds__(GN_THREADS) gn_stats_join(GnShape s, const float2* __restrict__ part, float eps,
                                                             float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-  const long long i = (long long)blockIdx.x * (GN_THREADS / 64) + (threadIdx.x >> 6);
+  const long long i = gn_block() * (GN_THREADS / 64) + (threadIdx.x >> 6);
   if (i >= s.samples * s.groups) return;
   const long long n = i / s.groups, g = i % s.groups;
   const int lane = threadIdx.x & 63;
@@ -258,7 +265,7 @@ __global__ void __launch_bounds__(GN_THREADS) gn_apply(GnShape s, const T* __res
                                                        const float* __restrict__ mean, const float* __restrict__ rstd,
                                                        T* __restrict__ y) {
   const GnPlace p = gn_place(s);
-  if (!p.active) return;
+  if (!p.active || p.n >= s.samples) return;
   for (int t = 0; t < s.tiles; ++t) {
     const int c = (t * s.vecs + p.j) * V;
     if (c >= s.width) break;
@@ -291,6 +298,7 @@ __global__ void __launch_bounds__(GN_THREADS) gn_sums(GnShape s, const T* __rest
                                                       const float* __restrict__ rstd, float2* __restrict__ part) {
   __shared__ float2 red[GN_THREADS * V];
   const GnPlace p = gn_place(s);
+  if (p.n >= s.samples) return;
   for (int t = 0; t < s.tiles; ++t) {
     const int c = (t * s.vecs + p.j) * V;
     float s1[V], s2[V];
@@ -344,8 +352,11 @@ __global__ void __launch_bounds__(GN_THREADS) gn_sums(GnShape s, const T* __rest
 #define GN_JOIN_THREADS 1024
 __global__ void __launch_bounds__(GN_JOIN_THREADS) gn_sums_columns(GnShape s, float2* __restrict__ part) {
   __shared__ float2 red[GN_JOIN_THREADS];
-  const int slabs = (s.channels + 63) / 64, c = (int)(blockIdx.x % slabs) * 64 + (threadIdx.x & 63), share = threadIdx.x >> 6;
-  float2* p = part + (long long)(blockIdx.x / slabs) * s.chunks * s.channels + c;
+  const int slabs = (s.channels + 63) / 64, share = threadIdx.x >> 6;
+  const long long n = gn_block() / slabs;
+  if (n >= s.samples) return;
+  const int c = (int)(gn_block() % slabs) * 64 + (threadIdx.x & 63);
+  float2* p = part + n * s.chunks * s.channels + c;
   float2 a = make_float2(0.0f, 0.0f);
   if (c < s.channels) {
 #pragma unroll 4
@@ -372,8 +383,9 @@ __global__ void __launch_bounds__(GN_THREADS) gn_sums_join(GnShape s, int chunks
                                                            GnParams q,
                                                            float2* __restrict__ ab) {
   __shared__ float2 red[GN_THREADS];
-  const long long n = blockIdx.x / s.groups;
-  const int g = (int)(blockIdx.x % s.groups), lane = threadIdx.x % across, share = threadIdx.x / across;
+  const long long pair = gn_block(), n = pair / s.groups;
+  if (n >= s.samples) return;
+  const int g = (int)(pair % s.groups), lane = threadIdx.x % across, share = threadIdx.x / across;
   const int shares = GN_THREADS / across;
   float2 t = make_float2(0.0f, 0.0f);  // this thread's part of A and B
   for (int base = 0; base < s.cpg; base += across) {
@@ -412,7 +424,7 @@ __global__ void __launch_bounds__(GN_THREADS) gn_sums_join(GnShape s, int chunks
     __syncthreads();
   }
   const float m = (float)s.length * (float)s.cpg;
-  if (threadIdx.x == 0) ab[blockIdx.x] = make_float2(red[0].x / m, red[0].y / m);
+  if (threadIdx.x == 0) ab[pair] = make_float2(red[0].x / m, red[0].y / m);
 }
 
 template <typename T, int V, int ACT>
@@ -420,7 +432,7 @@ __global__ void __launch_bounds__(GN_THREADS) gn_dx(GnShape s, const T* __restri
                                                     const float* __restrict__ mean, const float* __restrict__ rstd,
                                                     const float2* __restrict__ ab, T* __restrict__ dx) {
   const GnPlace p = gn_place(s);
-  if (!p.active) return;
+  if (!p.active || p.n >= s.samples) return;
   for (int t = 0; t < s.tiles; ++t) {
     const int c = (t * s.vecs + p.j) * V;
     if (c >= s.width) break;
@@ -462,7 +474,7 @@ __global__ void __launch_bounds__(GN_PARAM_THREADS) gn_param_grads(int channels,
                                                                    void* __restrict__ dw, void* __restrict__ db) {
   constexpr int LANES = GN_PARAM_THREADS / GN_PARAM_CH;
   __shared__ double2 red[GN_PARAM_THREADS];
-  const int c = blockIdx.x * GN_PARAM_CH + threadIdx.x % GN_PARAM_CH;
+  const long long c = gn_block() * GN_PARAM_CH + threadIdx.x % GN_PARAM_CH;
   const int lane = threadIdx.x / GN_PARAM_CH;
   double2 t = make_double2(0.0, 0.0);
   if (c < channels) {
@@ -562,9 +574,10 @@ __global__ void __launch_bounds__(THREADS) gn_tile_forward(GnTile q, const T* __
   float* buf = lds;                                    // [THREADS * GN_EACH]
   float2* stat = (float2*)(lds + THREADS * GN_EACH);   // [per * groups]
   float2* wb = stat + q.per * q.groups;                // [channels]
+  const long long first = gn_block() * q.per;
+  if (first >= q.samples) return;
   for (int c = threadIdx.x; c < q.channels; c += THREADS)
     wb[c] = make_float2(gn_param<T>(par.w, par.f32, c, 1.0f), gn_param<T>(par.b, par.f32, c, 0.0f));
-  const long long first = (long long)blockIdx.x * q.per;
   const int here = q.samples - first < q.per ? (int)(q.samples - first) : q.per;
   const int values = here * q.values;
   const long long base = first * q.values;
@@ -756,7 +769,7 @@ __global__ void __launch_bounds__(GN_THREADS) gn_rows_forward(GnRows q, const T*
     b[i] = gn_param<T>(par.b, par.f32, c + i, 0.0f);
   }
   const float inv = 1.0f / (float)(q.span * V);
-  const long long base = (long long)blockIdx.x * GN_THREADS * GN_ROW_STEPS + threadIdx.x;
+  const long long base = gn_block() * GN_THREADS * GN_ROW_STEPS + threadIdx.x;
   float v[GN_ROW_STEPS][V];
 #pragma unroll
   for (int k = 0; k < GN_ROW_STEPS; ++k)
@@ -904,8 +917,20 @@ GnShape gn_shape(long long samples, long long length, int channels, int groups, 
   return s;
 }
 
+// `blocks` workgroups as gn_block counts them
+dim3 gn_grid(long long blocks) {
+  if (blocks <= GN_GRID_X) return dim3((unsigned)blocks);
+  return dim3(GN_GRID_X, (unsigned)((blocks + GN_GRID_X - 1) / GN_GRID_X));
+}
+const long long GN_BLOCKS_MOST = 65535LL * GN_GRID_X;  // (a grid's second dimension has 16 bits)
+
 const size_t GN_LDS = 152 * 1024;  // of a workgroup's 160 KB
 const int GN_TILE_BLOCKS = 1024;  // workgroups of the one-pass backward kernels: one record of column sums each
+
+// the largest of the launches for these samples: slabs and chunks, groups, or columns of 64 channels
+long long gn_blocks(const GnShape& s) {
+  return s.samples * std::max((long long)s.slabs * s.chunks, std::max((long long)s.groups, (s.channels + 63LL) / 64));
+}
 
 bool gn_tile(long long samples, long long length, int channels, int groups, int v, int most, GnTile& q) {
   if (length * channels > most) return false;
@@ -1018,14 +1043,14 @@ void gn_forward(const GnShape& s, const void* x, GnParams q, float eps, int act,
   GnRows rows;
   if (gn_rows(s, V, rows)) {
     const long long per = GN_THREADS * GN_ROW_STEPS;
-    GN_ACTS(act, gn_rows_forward, T, V, dim3((unsigned)((rows.vectors + per - 1) / per)), dim3(GN_THREADS), 0, st, rows,
+    GN_ACTS(act, gn_rows_forward, T, V, gn_grid((rows.vectors + per - 1) / per), dim3(GN_THREADS), 0, st, rows,
             (const T*)x, q, eps, mean, rstd, (T*)y)
     return;
   }
   GnTile tile;
   if (const int threads = gn_tile_threads(s.samples, s.length, s.channels, s.groups, V, false, tile)) {
     const size_t lds = gn_tile_lds(tile, threads, false);
-    const dim3 tiles((unsigned)((s.samples + tile.per - 1) / tile.per));
+    const dim3 tiles = gn_grid((s.samples + tile.per - 1) / tile.per);
     if (threads == 256) {
       GN_TILE_ACTS(act, gn_tile_forward, T, V, 256, lds, tiles, dim3(256), lds, st, tile, (const T*)x, q, eps, mean, rstd, (T*)y)
     } else {
@@ -1033,10 +1058,10 @@ void gn_forward(const GnShape& s, const void* x, GnParams q, float eps, int act,
     }
     return;
   }
-  const dim3 grid((unsigned)(s.samples * s.slabs * s.chunks)), block(GN_THREADS);
+  const dim3 grid = gn_grid(s.samples * s.slabs * s.chunks), block(GN_THREADS);
   hipLaunchKernelGGL((gn_stats<T, V>), grid, block, 0, st, s, (const T*)x, part);
   const long long pairs = s.samples * s.groups;
-  hipLaunchKernelGGL(gn_stats_join, dim3((unsigned)((pairs + GN_THREADS / 64 - 1) / (GN_THREADS / 64))), block, 0, st, s, part, eps, mean,
+  hipLaunchKernelGGL(gn_stats_join, gn_grid((pairs + GN_THREADS / 64 - 1) / (GN_THREADS / 64)), block, 0, st, s, part, eps, mean,
                      rstd);
   GN_ACTS(act, gn_apply, T, V, grid, block, 0, st, s, (const T*)x, q, mean, rstd, (T*)y)
 }
@@ -1047,7 +1072,7 @@ void gn_backward(const GnShape& s, const void* x, const void* dy, GnParams q, in
   const bool sums = dw != nullptr || db != nullptr;
   auto params = [&](long long count, long long stride) {
     if (sums)
-      hipLaunchKernelGGL((gn_param_grads<T>), dim3((unsigned)((s.channels + GN_PARAM_CH - 1) / GN_PARAM_CH)),
+      hipLaunchKernelGGL((gn_param_grads<T>), gn_grid((s.channels + GN_PARAM_CH - 1LL) / GN_PARAM_CH),
                          dim3(GN_PARAM_THREADS), 0, st, s.channels, count, stride, part, q.f32, dw, db);
   };
   GnRows rows;
@@ -1066,16 +1091,16 @@ void gn_backward(const GnShape& s, const void* x, const void* dy, GnParams q, in
                  mean, rstd, (T*)dx, sums ? part : nullptr)
     return params(blocks, s.channels);
   }
-  const dim3 grid((unsigned)(s.samples * s.slabs * s.chunks)), block(GN_THREADS);
+  const dim3 grid = gn_grid(s.samples * s.slabs * s.chunks), block(GN_THREADS);
   GN_ACTS(act, gn_sums, T, V, grid, block, 0, st, s, (const T*)x, (const T*)dy, q, mean, rstd, part)
   const long long pairs = s.samples * s.groups;
   int across = 1;
   while (across < GN_THREADS && across < s.cpg) across *= 2;
   const bool wide = s.cpg > 64 && s.chunks > 1;
   if (wide)
-    hipLaunchKernelGGL(gn_sums_columns, dim3((unsigned)(s.samples * ((s.channels + 63) / 64))), dim3(GN_JOIN_THREADS), 0, st, s,
+    hipLaunchKernelGGL(gn_sums_columns, gn_grid(s.samples * ((s.channels + 63) / 64)), dim3(GN_JOIN_THREADS), 0, st, s,
                        part);
-  hipLaunchKernelGGL((gn_sums_join<T>), dim3((unsigned)pairs), block, 0, st, s, wide ? 1 : s.chunks, across, part, q, ab);
+  hipLaunchKernelGGL((gn_sums_join<T>), gn_grid(pairs), block, 0, st, s, wide ? 1 : s.chunks, across, part, q, ab);
   if (dx != nullptr) {
     GN_ACTS(act, gn_dx, T, V, grid, block, 0, st, s, (const T*)x, (const T*)dy, q, mean, rstd, ab, (T*)dx)
   }
@@ -1109,7 +1134,7 @@ extern "C" NSA_API int nsa_group_norm_forward(long long samples, long long lengt
     return nsa_fail(NSA_E_ARG, "%s: workspace too small", what);
   int v;
   const GnShape s = gn_shape(samples, length, channels, groups, nsa_elem_bytes(dtype), (uintptr_t)x_dev | (uintptr_t)y_dev, v);
-  if (s.samples * s.slabs * s.chunks >= (1LL << 31)) return nsa_fail(NSA_E_ARG, "%s: too many samples", what);
+  if (gn_blocks(s) > GN_BLOCKS_MOST) return nsa_fail(NSA_E_ARG, "%s: too many samples", what);
   const GnParams q = {weight_dev, bias_dev, weight_dtype == NSA_DT_F32};
   hipStream_t st = (hipStream_t)stream;
   float2* part = (float2*)workspace_dev;
@@ -1130,7 +1155,7 @@ extern "C" NSA_API int nsa_group_norm_backward(long long samples, long long leng
   const int f32 = weight_dtype == NSA_DT_F32;
   if (samples == 0 || length == 0) {  // no rows: the parameters' gradients are zero
     if (dweight_dev == nullptr && dbias_dev == nullptr) return NSA_OK;
-    hipLaunchKernelGGL((gn_param_grads<nsa_f16>), dim3((unsigned)((channels + GN_PARAM_CH - 1) / GN_PARAM_CH)),
+    hipLaunchKernelGGL((gn_param_grads<nsa_f16>), gn_grid((channels + GN_PARAM_CH - 1LL) / GN_PARAM_CH),
                        dim3(GN_PARAM_THREADS), 0, st, channels, 0LL, 0LL, (const float2*)nullptr, f32, dweight_dev, dbias_dev);  // (zero has the same bits in both 16-bit types)
     return gn_done(what);
   }
@@ -1140,7 +1165,7 @@ extern "C" NSA_API int nsa_group_norm_backward(long long samples, long long leng
   int v;
   const GnShape s = gn_shape(samples, length, channels, groups, nsa_elem_bytes(dtype),
                              (uintptr_t)x_dev | (uintptr_t)dy_dev | (uintptr_t)dx_dev, v);
-  if (s.samples * s.slabs * s.chunks >= (1LL << 31)) return nsa_fail(NSA_E_ARG, "%s: too many samples", what);
+  if (gn_blocks(s) > GN_BLOCKS_MOST) return nsa_fail(NSA_E_ARG, "%s: too many samples", what);
   const GnParams q = {weight_dev, bias_dev, f32};
   GnTile tile;
   const bool chunked = gn_tile_threads(samples, length, channels, groups, v, true, tile) == 0;

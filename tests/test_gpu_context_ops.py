@@ -608,3 +608,83 @@ def test_group_norm_of_more_than_two_to_the_31_elements(shape):
     end = x.detach()[tail].clone().requires_grad_(True)
     (want,) = torch.autograd.grad(ops.group_norm_act(end, 8, activation="silu"), [end], y[tail].clone())
     assert float((dx[tail].double() - want.double()).norm()) <= (2 * u(torch.bfloat16) + 1e-4) * float(want.double().norm())
+
+
+# ---- launches of more workgroups than one dimension holds -------------------------------------------------------------
+
+
+def test_group_norm_of_more_than_two_to_the_24_groups_of_samples():
+    """8193 x 2048 (sample, group) pairs.  The first and last samples agree with themselves alone bit for bit: the same chunks.
+    bias: a float32 sum of 3 terms per sample, then 64 bits and a rounding.  weight: xh = (x - mean) rstd of three values; the
+    mean is off by 3 u max|x|, the root by twice that, so xh, of at most sqrt(3), by 16 u (1 + max|x| rstd)."""
+    shape, groups = (8193, 3, 2048), 2048
+    x, w, b, dy = _group_norm_case(shape, groups, torch.bfloat16, torch.float32, None)
+    leaves = [v.requires_grad_(True) for v in (x, w, b)]
+    y = ops.group_norm_act(x, groups, w, b)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    for part in (slice(0, 2), slice(-2, None)):
+        xs = x.detach()[part].clone().requires_grad_(True)
+        ys = ops.group_norm_act(xs, groups, w, b)
+        assert torch.equal(ys, y[part])
+        assert torch.equal(torch.autograd.grad(ys, [xs], dy[part].clone())[0], dx[part])
+    assert torch.isfinite(dx).all()
+    d, v = dy.double(), x.detach().double()
+    rstd = 1 / torch.sqrt(v.var(1, correction=0, keepdim=True) + 1e-5)
+    xh = (v - v.mean(1, keepdim=True)) * rstd
+    assert bool(((db.double() - d.sum((0, 1))).abs() <= 4 * U32 * d.abs().sum((0, 1))).all())
+    tol = (d.abs() * 16 * U32 * (1 + v.abs().amax(1, keepdim=True) * rstd)).sum((0, 1))
+    assert bool(((dw.double() - (d * xh).sum((0, 1))).abs() <= tol + U32 * dw.abs()).all())
+
+
+def test_group_norm_of_more_than_two_to_the_24_slabs():
+    """A prime number of groups of one channel: 2056 x 8209 workgroups of one channel each, in every pass."""
+    shape, groups = (2056, 2, 8209), 8209
+    x, w, b, dy = _group_norm_case(shape, groups, torch.bfloat16, torch.float32, None)
+    leaves = [v.requires_grad_(True) for v in (x, w, b)]
+    y = ops.group_norm_act(x, groups, w, b, activation="silu")
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    for part in (slice(0, 1), slice(-1, None)):
+        xs = x.detach()[part].clone().requires_grad_(True)
+        ys = ops.group_norm_act(xs, groups, w, b, activation="silu")
+        assert torch.equal(ys, y[part])
+        assert torch.equal(torch.autograd.grad(ys, [xs], dy[part].clone())[0], dx[part])
+    # of two values, xh is their difference over its own size: 1 / sqrt(1 + eps / var), by the formula of the tests above
+    v, d = x.detach().double(), dy.double()
+    rstd = 1 / torch.sqrt(v.var(1, correction=0, keepdim=True) + 1e-5)
+    xh = (v - v.mean(1, keepdim=True)) * rstd
+    z = xh * w.detach().double() + b.detach().double()
+    s = torch.sigmoid(z)
+    dz, lost = d * s * (1 + z * (1 - s)), 16 * U32 * (1 + v.abs().amax(1, keepdim=True) * rstd)
+    # silu and its slope change by at most 1.1 and 0.5 times what z is off by; their own arithmetic loses less than 16 u (1 + |z|)
+    far = w.detach().double().abs() * lost + 16 * U32 * (1 + z.abs())
+    assert bool(((y.double() - z * s).abs() <= u(torch.bfloat16) * (z * s).abs() + 1.2 * far + smallest(torch.bfloat16)).all())
+    size = (d.abs() * (far + lost)).sum((0, 1))
+    assert bool(((db.double() - dz.sum((0, 1))).abs() <= size).all()) and bool(((dw.double() - (dz * xh).sum((0, 1))).abs() <= 2 * size).all())
+
+
+def test_group_norm_launches_in_two_dimensions():
+    """More than 2^20 workgroups of rows (one element a lane: an odd address) and of samples in tiles, and of channels."""
+    rows = 2**24 + 4097
+    room = torch.empty(rows * 64 + 1, dtype=torch.bfloat16, device=DEV).normal_(generator=torch.Generator(device=DEV).manual_seed(3))
+    x = room[1:].view(rows, 64)
+    y = ops.group_norm_act(x, 8, activation="silu")
+    for part in (slice(0, 1000), slice(-5000, None)):
+        alone = ops.group_norm_act(x[part].clone(), 8, activation="silu")
+        # (16-byte accesses there: another order of 8 additions)
+        assert float((y[part].double() - alone.double()).norm()) <= (2 * u(torch.bfloat16) + 128 * U32) * float(alone.double().norm())
+    del room, x, y
+    samples = 2**20 + 5
+    x = torch.empty(samples, 4100, dtype=torch.bfloat16, device=DEV).normal_(generator=torch.Generator(device=DEV).manual_seed(4))
+    y = ops.group_norm_act(x, 41, activation="tanh")
+    for part in (slice(0, 3), slice(2**20 - 1, None)):
+        assert torch.equal(ops.group_norm_act(x[part].clone(), 41, activation="tanh"), y[part])
+    del x, y
+    c = 2**24 + 1024
+    x, dy = randn(2, c, seed=5), randn(2, c, seed=6)
+    w, b = torch.ones(c, device=DEV, requires_grad=True), torch.zeros(c, device=DEV, requires_grad=True)
+    dw, db = torch.autograd.grad(ops.group_norm_act(x, 64, w, b), [w, b], dy)
+    v, d = x.double().view(2, 64, -1), dy.double()
+    xh = ((v - v.mean(2, keepdim=True)) / torch.sqrt(v.var(2, correction=0, keepdim=True) + 1e-5)).view(2, c)
+    # (two terms; a chain of 257 values in a thread's sums, about a member of at most 6 spreads)
+    assert bool(((db.double() - d.sum(0)).abs() <= 2 * U32 * d.abs().sum(0)).all())
+    assert bool(((dw.double() - (d * xh).sum(0)).abs() <= 260 * U32 * (1 + 6) * (d.abs() * (1 + xh.abs())).sum(0)).all())
