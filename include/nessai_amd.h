@@ -659,7 +659,7 @@ NSA_API int nsa_grad_clip(int count, void* const* tensors, const long long* size
                           float max_norm, void* workspace_dev, size_t workspace_bytes, float* norm_out_dev, void* stream);
 
 /* Group norm with an activation, channels last: x [samples][length][channels], groups of channels / groups neighbouring
- * channels, mean and (biased) variance over a sample's positions and a group's channels,
+ * channels (at most 2^30 of them), mean and (biased) variance over a sample's positions and a group's channels,
  *   y = act(((x - mean) / sqrt(var + eps)) * weight[c] + bias[c]).
  * weight_dev / bias_dev: [channels] of type weight_dtype (float32 or x's type), or NULL.  mean_dev / rstd_dev:
  * [samples][groups] float32, written by the forward call and read by the backward call.  The backward call writes the

@@ -1002,6 +1002,8 @@ int gn_check(const char* what, long long samples, long long length, int channels
              int activation) {
   if (samples < 0 || length < 0 || channels < 1 || groups < 1 || channels % groups != 0)
     return nsa_fail(NSA_E_ARG, "%s: bad shape (channels must be a multiple of groups)", what);
+  // (channels are counted in 32 bits, in steps of a workgroup that run past the last one)
+  if (channels > (1 << 30)) return nsa_fail(NSA_E_ARG, "%s: at most 2^30 channels", what);
   if (!nsa_elem_known(dtype)) return nsa_fail(NSA_E_ARG, "%s: unknown type %d", what, dtype);
   if (weight_dtype != NSA_DT_F32 && weight_dtype != dtype)
     return nsa_fail(NSA_E_ARG, "%s: weight and bias are float32 or of x's type", what);

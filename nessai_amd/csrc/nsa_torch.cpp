@@ -164,8 +164,9 @@ Tensor group_norm_act(const Tensor& x_, int64_t groups, const std::optional<Tens
   TORCH_CHECK_VALUE(x_.dim() >= 2, "expected a tensor of shape (N, ..., C), got ", x_.sizes());
   dtype_code(x_, "group_norm_act: x");
   const int64_t channels = x_.size(-1);
-  TORCH_CHECK_VALUE(groups >= 1 && channels >= 1 && channels % groups == 0 && channels < (1LL << 31), channels,
+  TORCH_CHECK_VALUE(groups >= 1 && channels >= 1 && channels % groups == 0, channels,
                     " channels cannot be divided into ", groups, " groups");
+  TORCH_CHECK_VALUE(channels <= (1 << 30), "group_norm_act: at most 2**30 channels (got ", channels, ")");
   TORCH_CHECK_VALUE(eps >= 0.0, "eps must not be negative (got ", eps, ")");
   Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
   for (const Tensor* t : {&x_, &std::as_const(weight), &std::as_const(bias)}) no_tangent(*t, "group_norm_act");

@@ -35,7 +35,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation=N
     ``num_groups`` groups of ``C / num_groups`` neighbouring channels, over all positions between the first and the
     last dimension.  ``weight`` / ``bias``: ``(C,)``, float32 or of ``x``'s type, or ``None``.  ``activation``:
     ``None``, ``"relu"``, ``"tanh"`` or ``"silu"``, as the flows' conditioners have them.  Differentiable once in ``x``,
-    ``weight`` and ``bias``.  A tensor that is not contiguous is copied first; the result is contiguous.
+    ``weight`` and ``bias``.  A tensor that is not contiguous is copied first; the result is contiguous.  At most ``2**30``
+    channels.
     """
     if activation not in _ACTIVATIONS:
         raise ValueError(f"Unknown activation: {activation}")

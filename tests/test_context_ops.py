@@ -143,3 +143,25 @@ def test_entry_points_check_their_arguments_before_anything_is_launched():
     assert L.nsa_embedding_backward(4, 4, 8, 0, ws, 8, ws, 1.0, -1, ws, ws, 0, None) < 0
     assert b"workspace" in L.nsa_last_error()
     assert L.nsa_embedding_backward(4, 4, 8, 0, ws, 8, None, 1.0, -1, ws, ws, 1 << 20, None) < 0
+
+
+def test_group_norm_refuses_channels_that_its_counters_do_not_hold():
+    """A group of 2^31 - 1 channels, walked in steps of 256, would pass the last 32-bit number."""
+    L, ws = lib.load(), 4096  # (an address that no call below reaches)
+    for channels in (2**30 + 1, 2**31 - 1):
+        assert L.nsa_group_norm_forward(1, 1, channels, 1, 1, ws, 0, None, None, 1e-5, -1, ws, ws, ws, ws, 1 << 40, None) < 0
+        assert b"2^30 channels" in L.nsa_last_error()
+        assert L.nsa_group_norm_backward(1, 1, channels, 1, 1, ws, ws, 0, None, None, -1, ws, ws, ws, None, None, ws, 1 << 40, None) < 0
+        assert b"2^30 channels" in L.nsa_last_error()
+    x = torch.empty(1, dtype=torch.bfloat16).expand(2, 2**30 + 1)
+    with pytest.raises(ValueError, match="channels"):
+        ops.group_norm_act(x, 1)
+
+
+def test_group_norm_refuses_more_workgroups_than_a_launch_holds():
+    L, ws = lib.load(), 4096
+    samples, channels = 2**32, 8209  # (a prime number of groups: a workgroup each, in every sample)
+    assert L.nsa_group_norm_forward(samples, 1, channels, channels, 1, ws, 0, None, None, 1e-5, -1, ws, ws, ws, ws, 1 << 62, None) < 0
+    assert b"too many samples" in L.nsa_last_error()
+    assert L.nsa_group_norm_backward(samples, 1, channels, channels, 1, ws, ws, 0, None, None, -1, ws, ws, ws, None, None, ws, 1 << 62, None) < 0
+    assert b"too many samples" in L.nsa_last_error()
