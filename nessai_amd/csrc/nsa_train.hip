@@ -42,7 +42,7 @@ __device__ __forceinline__ float tr_act_grad(float x, int act) {
   return s * (1.0f + x * (1.0f - s));
 }
 
-// Y[n][O] = act_in(X[:, cols])[n][I] . W[O][I]^T + b (+ R)
+// Y[n][O] = act_in(X[:, cols])[n][I] . W[O][I]^T + b (+ R); b may be null (no bias)
 // M (optional, [n][I]): a multiplier of the activated input - the dropout mask of this product's input
 // (0 or 1 / (1 - p): tr_dropout_mask), training mode only
 __global__ void __launch_bounds__(64) tr_gemm_nt(int n, int I, int O, const float* __restrict__ X, int ldx,
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(64) tr_gemm_nt(int n, int I, int O, const floa
   for (int r = 0; r < 16; ++r) {
     const int o = col0 + (r & 3) + 8 * (r >> 2) + 4 * half;
     if (o < O && row < n) {
-      float v = acc[r] + b[o];
+      float v = acc[r] + (b ? b[o] : 0.0f);
       if (R) v += R[(long long)row * ldy + o];
       Y[(long long)row * ldy + o] = v;
     }
@@ -2166,13 +2166,11 @@ static void tr_forward(const long long* plan, const int* tabs, float* params, co
                            (unsigned*)(q.vec + 4 * D));
         continue;
       }
-      float* zero = q.vec;  // zero bias for the first product
-      (void)hipMemsetAsync(zero, 0, D * sizeof(float), s);
       hipLaunchKernelGGL(tr_lu_build, blocks_for(D * D), dim3(256), 0, s, D, params + r[2], params + r[3],
                          params + r[4], eps, q.Lm, q.Um, w.scal + 1);
       hipLaunchKernelGGL(tr_gather_cols, blocks_for(n * D), dim3(256), 0, s, (int)n, D, w.x, D, cols, q.xin, 0);
       hipLaunchKernelGGL(tr_gemm_nt, tiles(n, D), dim3(64), 0, s, (int)n, D, D, q.xin, D, (const int*)nullptr,
-                         ACT_NONE, q.Um, zero, (const float*)nullptr, q.t, D);
+                         ACT_NONE, q.Um, (const float*)nullptr, (const float*)nullptr, q.t, D);
       hipLaunchKernelGGL(tr_gemm_nt, tiles(n, D), dim3(64), 0, s, (int)n, D, D, q.t, D, (const int*)nullptr,
                          ACT_NONE, q.Lm, params + r[5], (const float*)nullptr, w.x, D);
     } else if (r[0] == TR_SVD) {
@@ -2629,7 +2627,7 @@ static int tr_backward_impl(const long long* plan, const int* tables_dev, const 
   const long long D = plan[0], n_params = plan[8];
   TrWs w;
   tr_carve(plan, n, workspace_dev, w);
-  // (a kernel, not hipMemsetAsync: these launches may be captured into a graph)
+  // (a kernel, not a memset: these launches may be captured into a graph)
   hipLaunchKernelGGL(tr_fill_zero, blocks_for(n_params), dim3(256), 0, s, n_params, grads_dev);
   if (gctx_out_dev != nullptr)
     hipLaunchKernelGGL(tr_fill_zero, blocks_for(n * plan[13]), dim3(256), 0, s, n * plan[13], gctx_out_dev);

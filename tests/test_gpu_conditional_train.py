@@ -40,6 +40,34 @@ def _train_pair(name, seed=3):
     return ref, flow, args[0], kw["context_features"]
 
 
+@pytest.mark.parametrize("training", [False, True], ids=["eval", "train"])
+@pytest.mark.parametrize("name", sorted(TRAIN_CASES))
+def test_captured_forward_replays(name, training):
+    """The layer-wise forward pass in a HIP graph, replayed between eager calls on other rows: ``z`` is the eager result every
+    time, bit for bit (no atomics on its way; batch statistics are read, not the running ones)."""
+    _, flow, D, C = _train_pair(name)
+    tr = flow.trainer()
+    x, c = torch.randn(400, D, device=DEV), torch.randn(400, C, device=DEV)
+    other = [torch.randn(300, D, device=DEV), torch.randn(300, C, device=DEV)]
+    with torch.no_grad():
+        want = tr.forward_saved(x, training, context=c)[0].clone()
+        if not training:
+            before = tr.forward_saved(other[0], False, context=other[1])[0].clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            z = tr.forward_saved(x, training, context=c)[0]
+        for _ in range(4):
+            z.fill_(float("nan"))
+            graph.replay()
+            eager = tr.forward_saved(other[0], training, context=other[1])[0]
+            torch.cuda.synchronize()
+            assert torch.equal(z, want)
+            assert training or torch.equal(eager, before)
+            torch.randn(1 << 20, device=DEV).mul_(3.0)
+            torch.cuda.synchronize()
+
+
 @pytest.mark.parametrize("name", sorted(TRAIN_CASES))
 def test_conditional_loss_and_gradients_match_autograd(name):
     """One minibatch of ``-mean(log_prob(x, context))`` (flowmodel/base.py:411-412): loss and every gradient - the
