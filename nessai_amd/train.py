@@ -485,6 +485,16 @@ def get_context_optimiser(flow_model):
     return flow_model._trainer
 
 
+def minibatch_bounds(n_rows, batch_size):
+    """Rows ``[a, b)`` of each minibatch.  A single row behind the last full one joins it: a pass in training mode needs two."""
+    if n_rows < 2:
+        raise ValueError(f"training needs at least two rows of data (got {n_rows})")
+    bounds = [(a, min(a + batch_size, n_rows)) for a in range(0, n_rows, batch_size)]
+    if len(bounds) > 1 and bounds[-1][1] - bounds[-1][0] == 1:
+        bounds[-2:] = [(bounds[-2][0], n_rows)]
+    return bounds
+
+
 def train_context_flow(flow_model, samples, max_epochs=None, patience=None, val_size=None, weights=None, conditional=None):
     """``train_flow`` of a flow with a net in front of its context: the reference's loop (flowmodel/base.py:400-452) over the
     parameters of both, through autograd.  The flow's forward and backward passes are the training kernels, the net's its own
@@ -499,6 +509,7 @@ def train_context_flow(flow_model, samples, max_epochs=None, patience=None, val_
     (x_train, c_train), (x_val, c_val), batch_size = flow_model.prep_data(
         samples, val_size=val_size, batch_size=tc["batch_size"], weights=weights, conditional=conditional
     )
+    bounds = minibatch_bounds(x_train.shape[0], batch_size)
     model = flow_model.model
     optimiser = get_context_optimiser(flow_model)
     max_epochs = tc["max_epochs"] if max_epochs is None else max_epochs
@@ -506,7 +517,6 @@ def train_context_flow(flow_model, samples, max_epochs=None, patience=None, val_
     base_lrs = [(tc.get("optimiser_kwargs") or {}).get("lr", tc["lr"])] * len(optimiser.param_groups)
     has_val = bool(validate and len(x_val))
     parameters, n_train = list(model.parameters()), x_train.shape[0]
-    bounds = [(a, min(a + batch_size, n_train)) for a in range(0, n_train, batch_size)]
     best_epoch, best_val_loss = 0, np.inf
     best = {k: v.detach().clone() for k, v in model.state_dict().items()}
     history = dict(loss=[], val_loss=[])

@@ -91,6 +91,20 @@ def test_proposals_refuse_a_context_net(tmp_path):
         ImportanceFlowModel(flow_config=config, output=str(tmp_path)).initialise()
 
 
+def test_minibatches_of_a_context_flow_have_two_rows_at_least():
+    from nessai_amd.train import minibatch_bounds
+
+    assert minibatch_bounds(91, 10) == [*((a, a + 10) for a in range(0, 80, 10)), (80, 91)]
+    for n in range(2, 60):
+        for size in range(2, 70):
+            bounds = minibatch_bounds(n, size)
+            assert bounds[0][0] == 0 and bounds[-1][1] == n and all(p[1] == q[0] for p, q in zip(bounds, bounds[1:]))
+            assert all(2 <= b - a <= size + 1 for a, b in bounds) and all(b - a == size for a, b in bounds[:-1])
+    for n in (0, 1):
+        with pytest.raises(ValueError, match="two rows"):
+            minibatch_bounds(n, 10)
+
+
 def test_training_launches_hold_no_memset():
     """They are captured into HIP graphs, where a memset node has given wrong results on later replays: memory is cleared by
     kernels."""

@@ -217,7 +217,28 @@ def test_labels_that_are_not_whole_numbers_show_in_their_rows():
 
 
 @pytest.mark.parametrize("ftype", ["nsf", "realnvp"])
-def test_flow_model_trains_a_context_flow(tmp_path, ftype):
+def test_flow_model_trains_where_one_row_is_left_over(tmp_path, ftype):
+    """91 rows in minibatches of 10, which the choice of a batch size accepts; and a training set of one row, refused."""
+    from nessai_amd.flowmodel import FlowModel
+
+    rng = np.random.default_rng(3)
+    labels = rng.integers(0, 3, size=(91, 1)).astype(float)
+    x = rng.normal(size=(91, 2)) + 2.0 * labels
+    config = dict(n_inputs=2, n_neurons=8, n_blocks=2, n_layers=1, ftype=ftype,
+                  context_net=dict(features=4, labels=[3], hidden_features=16))
+    training = dict(max_epochs=3, patience=10, lr=1e-3, batch_size=10, val_size=0.0)
+    fm = FlowModel(flow_config=config, training_config=training, output=str(tmp_path), rng=np.random.default_rng(1))
+    fm.initialise()
+    history = fm.train(x, conditional=labels)
+    assert fm._batch_size == 10 and len(history["loss"]) == 3 and np.isfinite(history["loss"]).all()
+    before = {k: v.clone() for k, v in fm.model.state_dict().items()}
+    with pytest.raises((ValueError, RuntimeError), match="two rows|batch size"):
+        fm.train(x[:1], conditional=labels[:1])
+    assert all(torch.equal(v, before[k]) for k, v in fm.model.state_dict().items())
+
+
+@pytest.mark.parametrize("ftype", ["nsf", "realnvp"])
+def test_flow_model_trains_a_context_flow_a_context_flow(tmp_path, ftype):
     """``FlowModel.train(conditional=...)`` of a flow with a context net runs, keeps the best weights, saves and reloads."""
     from nessai_amd.flowmodel import FlowModel
 
