@@ -177,6 +177,52 @@ def _expression(net, p, inputs):
     return h
 
 
+@pytest.mark.parametrize("kind", sorted(NETS))
+def test_three_steps_move_every_weight_as_plain_torch_does(kind):
+    """The weights after three clipped steps of AdamW, against float64.  A gradient is off by at most 2e-4 of its tensor's largest
+    (the gradient tests); where it is at least 0.02 of that in every step, so by 1 % of itself, the first step is the same to
+    rounding (lr times its sign) and the next two, ratios of running means, are off by at most 2 % of lr each: 0.1 lr is
+    allowed, where a weight that did not move, or moved the other way, is off by lr at least.  These are a third of the
+    weights or more.  Of the others, whose gradients' signs may differ, at most 2 % may be off by more than lr."""
+    lr = 1e-3
+    ref, flow, D, C = _pair("nsf_c2")
+    ref = ref.double().train()
+    torch.manual_seed(1)
+    net = ContextNet(C, **NETS[kind])
+    both = ContextFlow(flow, net)
+    both.to(DEV)
+    both.train()
+    opt = torch.optim.AdamW(both.parameters(), lr=lr)
+    _, p = _plain_net(net, _inputs(net, 2))
+    named_ref = {**{f"flow.{n}": q for n, q in ref.named_parameters()}, **{f"net.{n}": q for n, q in p.items()}}
+    start = {n: q.detach().clone() for n, q in named_ref.items()}
+    opt_ref = torch.optim.AdamW(list(named_ref.values()), lr=lr)
+    least = {n: torch.full_like(q, math.inf) for n, q in start.items()}
+    for step in range(3):
+        x, inputs = torch.randn(500, D, generator=torch.Generator().manual_seed(step)), _inputs(net, 500, seed=step)
+        opt.zero_grad()
+        (-both.log_prob(x.to(DEV), context=inputs.to(DEV)).mean()).backward()
+        ops.clip_grad_norm_(both.parameters(), 0.5)
+        opt.step()
+        opt_ref.zero_grad()
+        (-ref.log_prob(x.double(), context=_expression(net, p, inputs)).mean()).backward()
+        for n, q in named_ref.items():
+            g = q.grad.abs()
+            least[n] = torch.minimum(least[n], g / max(1e-3, float(g.max())))
+        torch.nn.utils.clip_grad_norm_(list(named_ref.values()), 0.5)
+        opt_ref.step()
+    named = dict(both.named_parameters())
+    assert sorted(named) == sorted(named_ref)
+    moved = total = others = far = 0
+    for n, q in named_ref.items():
+        off = (named[n].detach().cpu().double() - q.detach()).abs()
+        sure = least[n] >= 0.02
+        assert float(off[sure].max() if sure.any() else 0.0) <= 0.1 * lr, n
+        moved, total = moved + int(((q.detach() - start[n]).abs() > 0.5 * lr)[sure].sum()), total + off.numel()
+        others, far = others + int((~sure).sum()), far + int((off[~sure] > lr).sum())
+    assert moved >= 0.3 * total and far <= 0.02 * others, (moved, total, far, others)
+
+
 def test_methods_of_a_context_flow_agree():
     torch.manual_seed(2)
     both = ContextFlow(NeuralSplineFlow(4, 16, 2, 2, context_features=3), ContextNet(3, labels=[5], continuous=1))

@@ -404,6 +404,43 @@ def test_embedding_matches_the_definition(tokens, rows, width, how, ids_type, t)
     assert torch.equal(dw, again)
 
 
+# (tokens, rows, width, frequencies): every path of the gradient, runs over many chunks, tables of one to four sorting passes
+EXACT_TABLES = [
+    (1000, 6, 16, "uniform"), (50_001, 40, 64, "uniform"), (4096, 3000, 24, "uneven"), (4097, 70_001, 12, "uniform"),
+    (100_003, 5000, 7, "uneven"), (1_600_003, 3000, 4, "uniform"), (1_600_003, 20_000_000, 2, "uniform"),
+    (1_000_003, 5000, 64, "one"), (600_001, 300, 33, "one"), (300_001, 900, 40, "sorted"),
+]
+
+
+@pytest.mark.parametrize("t", TYPES, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("tokens,rows,width,how", EXACT_TABLES)
+def test_embedding_gradient_of_whole_numbers_is_exact(tokens, rows, width, how, t):
+    """Upstream values of at most 3 in magnitude and at most a million tokens in a row: every sum is a whole number below
+    2^24, exact in float32 in any order, so that one token lost, doubled or misplaced shows.  One rounding to the type."""
+    ids = _ids(tokens, rows, how, torch.int64)
+    dy = torch.randint(-3, 4, (tokens, width), generator=torch.Generator().manual_seed(7)).to(DEV)
+    dy[:, 0] = 1 + torch.arange(tokens, device=DEV) % 3  # (a column that cannot cancel)
+    w = torch.zeros(rows, width, dtype=t, device=DEV, requires_grad=True)
+    padding = rows // 3 if how == "uneven" else None
+    (dw,) = torch.autograd.grad(ops.embedding(ids, w, scale=0.25, padding_idx=padding), [w], dy.to(t))
+    want = torch.zeros(rows, width, dtype=torch.int64, device=DEV).index_add_(0, ids, dy)
+    if padding is not None:
+        want[padding] = 0
+    assert int(want.abs().max()) < 2**24
+    assert torch.equal(dw, (want.float() * 0.25).to(t))
+
+
+def test_embedding_of_a_transposed_table():
+    w = randn(11, 8, seed=1)
+    ids = torch.randint(0, 8, (3, 4, 5), generator=torch.Generator().manual_seed(2)).to(DEV)
+    leaf = w.clone().requires_grad_(True)
+    out = ops.embedding(ids, leaf.t())  # 8 rows of 11
+    assert torch.equal(out.detach(), w.t()[ids])
+    dy = torch.randint(-3, 4, (3, 4, 5, 11), generator=torch.Generator().manual_seed(3)).float().to(DEV)
+    (dw,) = torch.autograd.grad(out, [leaf], dy)
+    assert torch.equal(dw, torch.zeros(8, 11, device=DEV).index_add_(0, ids.reshape(-1), dy.reshape(-1, 11)).t())
+
+
 def test_embedding_of_indices_outside_the_table():
     """Such a row is NaN, takes no part in the gradient, and leaves every other row as it is."""
     w = randn(10, 6, seed=1).requires_grad_(True)
