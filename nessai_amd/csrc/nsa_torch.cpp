@@ -3,16 +3,22 @@
 // group norm runs for 5 us on the device and took 130 us, forward and backward, with the checks, allocations and the
 // autograd node in Python; clipping 300 gradients spent 220 us reading their attributes.
 //
-// Nothing here computes: arguments are checked, results and workspaces allocated, and one entry point called on the current
-// stream of the tensors' device.  The entry points' addresses come from the loaded libnessai_amd.so (nessai_amd/lib.py).
+// Nothing here computes.  The public operators check their arguments and record for autograd; each calls one of the inner
+// ones (a leading underscore), which exist for the CUDA (ROCm) dispatch key - results and workspaces are allocated and one
+// entry point called on the current stream of the tensors' device - and for the Meta key, where they return the results'
+// shapes.  The public ones have one body for every key, so a tracer (torch.compile, make_fx) sees the inner ones.
+// The entry points' addresses come from the loaded libnessai_amd.so (nessai_amd/lib.py).
 #include <ATen/ATen.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <array>
 #include <cmath>
 #include <optional>
+#include <tuple>
 #include <utility>
 #include <vector>
 
@@ -61,13 +67,28 @@ int dtype_code(const Tensor& t, const char* what) {
 }
 
 void on_device(const Tensor& t, const char* what) {
-  TORCH_CHECK(t.is_cuda(), what, ": nessai_amd operators take tensors on a ROCm device (got ", t.device(),
+  TORCH_CHECK(t.is_cuda() || t.is_meta(), what, ": nessai_amd operators take tensors on a ROCm device (got ", t.device(),
               "); there is no CPU fallback");
 }
 
 Tensor workspace(const Tensor& like, size_t bytes) {
   return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
 }
+
+// An inner operator, looked up once by its caller.  Called below autograd's keys: its fallback for operators without a
+// derivative puts the arguments on a stack, 25 ns for each tensor of a list.
+template <typename F>
+struct Inner {
+  c10::TypedOperatorHandle<F> handle;
+  explicit Inner(const char* name) : handle(c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>()) {}
+  template <typename... A>
+  auto operator()(A&&... a) const {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return handle.call(std::forward<A>(a)...);
+  }
+};
+
+std::optional<Tensor> given(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 
 const void* data(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* mutable_data(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
@@ -103,12 +124,19 @@ int param_dtype(const Tensor& weight, const Tensor& bias) {
   return p.defined() ? dtype_code(p, "group_norm_act: weight") : NSA_DT_F32;
 }
 
-Tensor group_norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups, double eps,
-                          int64_t activation, Tensor& stats) {
+std::tuple<Tensor, Tensor> group_norm_results(const Tensor& x, int64_t groups) {
+  return {at::empty(x.sizes(), x.options()), at::empty({2, Rows(x).samples, groups}, x.options().dtype(at::kFloat))};
+}
+
+// y, and the statistics: [mean, 1 / sqrt(var + eps)][sample][group]
+std::tuple<Tensor, Tensor> group_norm_forward(const Tensor& x, const std::optional<Tensor>& weight_,
+                                              const std::optional<Tensor>& bias_, int64_t groups, double eps,
+                                              int64_t activation) {
   const Rows r(x);
-  Tensor y = at::empty(x.sizes(), x.options());
-  stats = at::empty({2, r.samples, groups}, x.options().dtype(at::kFloat));
-  if (x.numel() == 0) return y;
+  const Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
+  auto results = group_norm_results(x, groups);
+  const auto& [y, stats] = results;
+  if (x.numel() == 0) return results;
   const c10::DeviceGuard guard(x.device());
   const int code = dtype_code(x, "group_norm_act: x");
   const size_t size = g_entry.group_norm_workspace(r.samples, r.length, r.channels, groups, code, 0);
@@ -118,15 +146,60 @@ Tensor group_norm_forward(const Tensor& x, const Tensor& weight, const Tensor& b
                                    data(weight), data(bias), (float)eps, activation, y.mutable_data_ptr(), mean,
                                    mean + r.samples * groups, ws.mutable_data_ptr(), size, stream_of(x)),
         "nsa_group_norm_forward");
-  return y;
+  return results;
+}
+
+std::tuple<Tensor, Tensor> group_norm_forward_meta(const Tensor& x, const std::optional<Tensor>&, const std::optional<Tensor>&,
+                                                   int64_t groups, double, int64_t) {
+  return group_norm_results(x, groups);
+}
+
+// dx, dweight, dbias: undefined where they are not wanted
+std::tuple<Tensor, Tensor, Tensor> group_norm_gradients(const Tensor& x, const std::optional<Tensor>& weight,
+                                                        const std::optional<Tensor>& bias, std::array<bool, 3> wanted) {
+  auto like = [](bool want, const std::optional<Tensor>& t) {
+    return want && t.has_value() ? at::empty(t->sizes(), t->options()) : Tensor();
+  };
+  return {like(wanted[0], x), like(wanted[1], weight), like(wanted[2], bias)};
+}
+
+std::tuple<Tensor, Tensor, Tensor> group_norm_backward(const Tensor& dy, const Tensor& x, const std::optional<Tensor>& weight_,
+                                                       const std::optional<Tensor>& bias_, const Tensor& stats,
+                                                       int64_t groups, int64_t activation, std::array<bool, 3> wanted) {
+  const Rows r(x);
+  const Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
+  const c10::DeviceGuard guard(x.device());
+  auto results = group_norm_gradients(x, weight_, bias_, wanted);
+  const auto& [dx, dw, db] = results;
+  const int code = dtype_code(x, "group_norm_act: x");
+  const size_t size = g_entry.group_norm_workspace(r.samples, r.length, r.channels, groups, code, 1);
+  const Tensor ws = workspace(x, size);
+  const float* mean = (const float*)stats.const_data_ptr();
+  check(g_entry.group_norm_backward(r.samples, r.length, r.channels, groups, code, data(x), data(dy),
+                                    param_dtype(weight, bias), data(weight), data(bias), activation, mean,
+                                    mean + r.samples * groups, mutable_data(dx), mutable_data(dw), mutable_data(db),
+                                    ws.mutable_data_ptr(), size, stream_of(x)),
+        "nsa_group_norm_backward");
+  return results;
+}
+
+std::tuple<Tensor, Tensor, Tensor> group_norm_backward_meta(const Tensor&, const Tensor& x, const std::optional<Tensor>& weight,
+                                                            const std::optional<Tensor>& bias, const Tensor&, int64_t, int64_t,
+                                                            std::array<bool, 3> wanted) {
+  return group_norm_gradients(x, weight, bias, wanted);
+}
+
+std::tuple<Tensor, Tensor> call_group_norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups,
+                                                   double eps, int64_t activation) {
+  static const Inner<decltype(group_norm_forward)> op("nessai_amd::_group_norm_forward");
+  return op(x, given(weight), given(bias), groups, eps, activation);
 }
 
 struct GroupNormAct : public torch::autograd::Function<GroupNormAct> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight_,
                         const std::optional<Tensor>& bias_, int64_t groups, double eps, int64_t activation) {
     const Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
-    Tensor stats;
-    Tensor y = group_norm_forward(x, weight, bias, groups, eps, activation, stats);
+    auto [y, stats] = call_group_norm_forward(x, weight, bias, groups, eps, activation);
     ctx->save_for_backward({x, weight, bias, stats});
     ctx->saved_data["groups"] = groups;
     ctx->saved_data["activation"] = activation;
@@ -135,26 +208,16 @@ struct GroupNormAct : public torch::autograd::Function<GroupNormAct> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("group_norm_act");
+    static const Inner<decltype(group_norm_backward)> op("nessai_amd::_group_norm_backward");
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[3];
-    const int64_t groups = ctx->saved_data["groups"].toInt(), activation = ctx->saved_data["activation"].toInt();
-    const Rows r(x);
-    const c10::DeviceGuard guard(x.device());
-    const Tensor dy = grads[0].contiguous();
-    Tensor dx, dw, db;
+    std::array<bool, 3> wanted = {};
     size_t edge = 0;  // of the tensors that were given, in order
-    if (ctx->needs_input_grad(edge++)) dx = at::empty(x.sizes(), x.options());
-    if (weight.defined() && ctx->needs_input_grad(edge++)) dw = at::empty(weight.sizes(), weight.options());
-    if (bias.defined() && ctx->needs_input_grad(edge++)) db = at::empty(bias.sizes(), bias.options());
-    const int code = dtype_code(x, "group_norm_act: x");
-    const size_t size = g_entry.group_norm_workspace(r.samples, r.length, r.channels, groups, code, 1);
-    const Tensor ws = workspace(x, size);
-    const float* mean = (const float*)stats.const_data_ptr();
-    check(g_entry.group_norm_backward(r.samples, r.length, r.channels, groups, code, data(x), data(dy),
-                                      param_dtype(weight, bias), data(weight), data(bias), activation, mean,
-                                      mean + r.samples * groups, mutable_data(dx), mutable_data(dw), mutable_data(db),
-                                      ws.mutable_data_ptr(), size, stream_of(x)),
-          "nsa_group_norm_backward");
+    wanted[0] = ctx->needs_input_grad(edge++);
+    wanted[1] = weight.defined() && ctx->needs_input_grad(edge++);
+    wanted[2] = bias.defined() && ctx->needs_input_grad(edge++);
+    auto [dx, dw, db] = op(grads[0].contiguous(), x, given(weight), given(bias), stats, ctx->saved_data["groups"].toInt(),
+                           ctx->saved_data["activation"].toInt(), wanted);
     return {dx, dw, db, Tensor(), Tensor(), Tensor()};
   }
 };
@@ -185,20 +248,20 @@ Tensor group_norm_act(const Tensor& x_, int64_t groups, const std::optional<Tens
                    "group_norm_act: weight and bias must have one type");
   on_device(x_, "group_norm_act");
   const Tensor x = x_.contiguous();
-  if (wants_grad({&x, &weight, &bias})) {
-    auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
-    return GroupNormAct::apply(x, given(weight), given(bias), groups, eps, activation);
-  }
-  Tensor stats;
-  return group_norm_forward(x, weight, bias, groups, eps, activation, stats);
+  if (wants_grad({&x, &weight, &bias})) return GroupNormAct::apply(x, given(weight), given(bias), groups, eps, activation);
+  return std::get<0>(call_group_norm_forward(x, weight, bias, groups, eps, activation));
 }
 
 // -- embedding --------------------------------------------------------------------------------------------------------
 
-Tensor embedding_forward(const Tensor& ids, const Tensor& weight, double scale) {
+Tensor embedding_rows(const Tensor& ids, const Tensor& weight, double) {
   std::vector<int64_t> shape = ids.sizes().vec();
   shape.push_back(weight.size(1));
-  Tensor out = at::empty(shape, weight.options());
+  return at::empty(shape, weight.options());
+}
+
+Tensor embedding_forward(const Tensor& ids, const Tensor& weight, double scale) {
+  Tensor out = embedding_rows(ids, weight, scale);
   if (out.numel() == 0) return out;
   const c10::DeviceGuard guard(weight.device());
   check(g_entry.embedding_forward(ids.numel(), weight.size(0), weight.size(1), dtype_code(weight, "embedding: weight"),
@@ -208,6 +271,27 @@ Tensor embedding_forward(const Tensor& ids, const Tensor& weight, double scale) 
   return out;
 }
 
+Tensor embedding_table(const Tensor& dy, const Tensor&, int64_t vocab, int64_t width, double, int64_t) {
+  return at::empty({vocab, width}, dy.options());
+}
+
+Tensor embedding_backward(const Tensor& dy, const Tensor& ids, int64_t vocab, int64_t width, double scale, int64_t padding) {
+  const c10::DeviceGuard guard(dy.device());
+  Tensor dweight = embedding_table(dy, ids, vocab, width, scale, padding);
+  const int code = dtype_code(dy, "embedding: weight");
+  const size_t size = g_entry.embedding_workspace(ids.numel(), vocab, width, code);
+  const Tensor ws = workspace(dy, size);
+  check(g_entry.embedding_backward(ids.numel(), vocab, width, code, data(ids), (int)ids.element_size(), data(dy), (float)scale,
+                                   padding, dweight.mutable_data_ptr(), ws.mutable_data_ptr(), size, stream_of(dy)),
+        "nsa_embedding_backward");
+  return dweight;
+}
+
+Tensor call_embedding_forward(const Tensor& ids, const Tensor& weight, double scale) {
+  static const Inner<decltype(embedding_forward)> op("nessai_amd::_embedding_forward");
+  return op(ids, weight, scale);
+}
+
 struct Embedding : public torch::autograd::Function<Embedding> {
   static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& ids, double scale, int64_t padding) {
     ctx->save_for_backward({ids});
@@ -215,23 +299,16 @@ struct Embedding : public torch::autograd::Function<Embedding> {
     ctx->saved_data["width"] = weight.size(1);
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding"] = padding;
-    return embedding_forward(ids, weight, scale);
+    return call_embedding_forward(ids, weight, scale);
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("embedding");
-    const Tensor ids = ctx->get_saved_variables()[0], dy = grads[0].contiguous();
-    const int64_t vocab = ctx->saved_data["vocab"].toInt(), width = ctx->saved_data["width"].toInt();
-    const c10::DeviceGuard guard(dy.device());
-    Tensor dweight = at::empty({vocab, width}, dy.options());
-    const int code = dtype_code(dy, "embedding: weight");
-    const size_t size = g_entry.embedding_workspace(ids.numel(), vocab, width, code);
-    const Tensor ws = workspace(dy, size);
-    check(g_entry.embedding_backward(ids.numel(), vocab, width, code, data(ids), (int)ids.element_size(), data(dy),
-                                     (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(),
-                                     dweight.mutable_data_ptr(), ws.mutable_data_ptr(), size, stream_of(dy)),
-          "nsa_embedding_backward");
-    return {dweight, Tensor(), Tensor(), Tensor()};
+    static const Inner<decltype(embedding_backward)> op("nessai_amd::_embedding_backward");
+    const Tensor ids = ctx->get_saved_variables()[0];
+    return {op(grads[0].contiguous(), ids, ctx->saved_data["vocab"].toInt(), ctx->saved_data["width"].toInt(),
+               ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt()),
+            Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -254,7 +331,7 @@ Tensor embedding(const Tensor& ids_, const Tensor& weight_, double scale, std::o
   TORCH_CHECK_VALUE(ids_.device() == weight_.device(), "embedding: indices are on ", ids_.device(), ", weight on ", weight_.device());
   on_device(weight_, "embedding");
   const Tensor ids = ids_.contiguous(), weight = weight_.contiguous();
-  return wants_grad({&weight}) ? Embedding::apply(weight, ids, scale, padding) : embedding_forward(ids, weight, scale);
+  return wants_grad({&weight}) ? Embedding::apply(weight, ids, scale, padding) : call_embedding_forward(ids, weight, scale);
 }
 
 // -- the norm over many gradients, and the clip -----------------------------------------------------------------------
@@ -269,8 +346,8 @@ void check_gradients(const std::vector<Tensor>& tensors, const char* what) {
   on_device(tensors[0], what);
 }
 
-// clip: by max_norm; otherwise the norm alone.  Every tensor fills one stretch of memory.
-Tensor norm_call(const std::vector<Tensor>& tensors, int64_t kind, bool clip, double max_norm) {
+// clip: by max_norm, in place; otherwise the norm alone.  Every tensor fills one stretch of memory.
+Tensor norm_call(at::TensorList tensors, int64_t kind, bool clip, double max_norm) {
   const c10::DeviceGuard guard(tensors[0].device());
   const int count = (int)tensors.size();
   std::vector<void*> places(count);
@@ -278,10 +355,11 @@ Tensor norm_call(const std::vector<Tensor>& tensors, int64_t kind, bool clip, do
   std::vector<int> codes(count);
   long long elements = 0;
   for (int i = 0; i < count; ++i) {
-    places[i] = const_cast<void*>(tensors[i].const_data_ptr());
-    sizes[i] = tensors[i].numel();
+    const Tensor& t = tensors[i];
+    places[i] = const_cast<void*>(t.const_data_ptr());
+    sizes[i] = t.numel();
     elements += sizes[i];
-    codes[i] = dtype_code(tensors[i], "gradients");
+    codes[i] = dtype_code(t, "gradients");
   }
   Tensor out = at::empty({}, tensors[0].options().dtype(at::kFloat));
   const size_t size = g_entry.grad_norm_workspace(count, elements);
@@ -297,6 +375,16 @@ Tensor norm_call(const std::vector<Tensor>& tensors, int64_t kind, bool clip, do
   return out;
 }
 
+Tensor total_norm(at::TensorList tensors, int64_t kind) { return norm_call(tensors, kind, false, 0.0); }
+Tensor clip_gradients(at::TensorList tensors, int64_t kind, double max_norm) { return norm_call(tensors, kind, true, max_norm); }
+Tensor total_norm_meta(at::TensorList tensors, int64_t) { return at::empty({}, tensors[0].options().dtype(at::kFloat)); }
+Tensor clip_gradients_meta(at::TensorList tensors, int64_t kind, double) { return total_norm_meta(tensors, kind); }
+
+Tensor call_total_norm(at::TensorList tensors, int64_t kind) {
+  static const Inner<decltype(total_norm)> op("nessai_amd::_total_norm");
+  return op(tensors, kind);
+}
+
 Tensor grad_norm(at::TensorList tensors, int64_t kind) {
   if (tensors.empty()) return at::zeros({}, at::kFloat);
   const at::NoGradGuard no_grad;
@@ -304,17 +392,13 @@ Tensor grad_norm(at::TensorList tensors, int64_t kind) {
   check_gradients(grads, "grad_norm: gradients");
   for (Tensor& g : grads)
     if (!g.is_non_overlapping_and_dense()) g = g.contiguous();
-  return norm_call(grads, kind, false, 0.0);
+  return call_total_norm(grads, kind);
 }
 
-Tensor clip_grad_norm(at::TensorList parameters, int64_t kind, double max_norm, bool error_if_nonfinite) {
+Tensor clip_(std::vector<Tensor> grads, int64_t kind, double max_norm, bool error_if_nonfinite) {
   TORCH_CHECK_VALUE(max_norm >= 0.0, "max_norm must not be negative or NaN (got ", max_norm, ")");
-  const at::NoGradGuard no_grad;
-  std::vector<Tensor> grads;
-  grads.reserve(parameters.size());
-  for (const Tensor& p : parameters)
-    if (p.grad().defined()) grads.push_back(p.grad());
   if (grads.empty()) return at::zeros({}, at::kFloat);
+  const at::NoGradGuard no_grad;
   check_gradients(grads, "clip_grad_norm_: gradients");
   // a gradient with gaps between its elements is clipped in a copy; one whose elements share memory cannot be
   std::vector<Tensor> dense = grads;
@@ -326,9 +410,10 @@ Tensor clip_grad_norm(at::TensorList parameters, int64_t kind, double max_norm, 
     g = g.contiguous();
   }
   if (error_if_nonfinite)
-    TORCH_CHECK(std::isfinite(norm_call(dense, kind, false, 0.0).item<float>()),
+    TORCH_CHECK(std::isfinite(call_total_norm(dense, kind).item<float>()),
                 "The total norm of the gradients from `parameters` is non-finite, so it cannot be clipped");
-  const Tensor norm = norm_call(dense, kind, true, max_norm);
+  static const Inner<decltype(clip_gradients)> op("nessai_amd::_clip_gradients_");
+  const Tensor norm = op(dense, kind, max_norm);
   for (size_t i = 0; i < grads.size(); ++i) {
     if (!dense[i].is_same(grads[i])) grads[i].copy_(dense[i]);
     // the kernels wrote behind torch's back: graphs that saved a gradient must see that it changed
@@ -337,14 +422,55 @@ Tensor clip_grad_norm(at::TensorList parameters, int64_t kind, double max_norm, 
   return norm;
 }
 
+Tensor clip_grad_norm(at::TensorList parameters, int64_t kind, double max_norm, bool error_if_nonfinite) {
+  std::vector<Tensor> grads;
+  grads.reserve(parameters.size());
+  for (const Tensor& p : parameters)
+    if (p.grad().defined()) grads.push_back(p.grad());
+  return clip_(std::move(grads), kind, max_norm, error_if_nonfinite);
+}
+
+// the same of the gradients themselves: a tracer, whose stand-ins for the parameters have no gradients, sees what changes
+Tensor clip_grad_norm_of(at::TensorList gradients, int64_t kind, double max_norm, bool error_if_nonfinite) {
+  return clip_(gradients.vec(), kind, max_norm, error_if_nonfinite);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(nessai_amd, m) {
   m.def("_bind_library(int[] addresses) -> ()", &bind_library);
   m.def("group_norm_act(Tensor x, int num_groups, Tensor? weight, Tensor? bias, float eps, int activation) -> Tensor",
         &group_norm_act);
+  m.def("_group_norm_forward(Tensor x, Tensor? weight, Tensor? bias, int num_groups, float eps, int activation) -> "
+        "(Tensor, Tensor)");
+  m.def("_group_norm_backward(Tensor dy, Tensor x, Tensor? weight, Tensor? bias, Tensor stats, int num_groups, "
+        "int activation, bool[3] wanted) -> (Tensor, Tensor, Tensor)");
   m.def("embedding(Tensor indices, Tensor weight, float scale, int? padding_idx) -> Tensor", &embedding);
+  m.def("_embedding_forward(Tensor indices, Tensor weight, float scale) -> Tensor");
+  m.def("_embedding_backward(Tensor dy, Tensor indices, int rows, int width, float scale, int padding) -> Tensor");
   m.def("grad_norm(Tensor[] tensors, int kind) -> Tensor", &grad_norm);
+  m.def("_total_norm(Tensor[] tensors, int kind) -> Tensor");
   m.def("clip_grad_norm_(Tensor[] parameters, int kind, float max_norm, bool error_if_nonfinite) -> Tensor",
         &clip_grad_norm);
+  m.def("clip_grad_norm_of_(Tensor(a!)[] gradients, int kind, float max_norm, bool error_if_nonfinite) -> Tensor",
+        &clip_grad_norm_of);
+  m.def("_clip_gradients_(Tensor(a!)[] gradients, int kind, float max_norm) -> Tensor");
+}
+
+TORCH_LIBRARY_IMPL(nessai_amd, CUDA, m) {
+  m.impl("_group_norm_forward", &group_norm_forward);
+  m.impl("_group_norm_backward", &group_norm_backward);
+  m.impl("_embedding_forward", &embedding_forward);
+  m.impl("_embedding_backward", &embedding_backward);
+  m.impl("_total_norm", &total_norm);
+  m.impl("_clip_gradients_", &clip_gradients);
+}
+
+TORCH_LIBRARY_IMPL(nessai_amd, Meta, m) {
+  m.impl("_group_norm_forward", &group_norm_forward_meta);
+  m.impl("_group_norm_backward", &group_norm_backward_meta);
+  m.impl("_embedding_forward", &embedding_rows);
+  m.impl("_embedding_backward", &embedding_table);
+  m.impl("_total_norm", &total_norm_meta);
+  m.impl("_clip_gradients_", &clip_gradients_meta);
 }

@@ -15,7 +15,8 @@ Values are float32, bfloat16 or float16; sums and statistics are held in float32
 There is no CPU implementation; float64 is refused, never cast down.  Derivatives are first-order and reverse-mode: a tensor
 with a tangent (``torch.autograd.forward_ad``, ``torch.func.jvp``) is refused.  Every call enqueues on the current stream of the
 tensors' device, waits for nothing (but ``error_if_nonfinite``) and may be captured into a HIP graph.  The functions here name
-the arguments; ``csrc/nsa_torch.cpp`` checks them, allocates and records for autograd.
+the arguments; ``csrc/nsa_torch.cpp`` checks them, allocates and records for autograd.  Meta and fake tensors give the results'
+shapes, so that the operators can be traced (``torch.compile``; the first call loads the library and is made outside).
 """
 
 import math
@@ -81,4 +82,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     """
     lib.load_torch()
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    return torch.ops.nessai_amd.clip_grad_norm_(parameters, _norm_code(norm_type), max_norm, error_if_nonfinite)
+    args = (_norm_code(norm_type), max_norm, error_if_nonfinite)
+    if torch.compiler.is_compiling():  # (the gradients as arguments: the compiled graph must show what changes)
+        return torch.ops.nessai_amd.clip_grad_norm_of_([p.grad for p in parameters if p.grad is not None], *args)
+    return torch.ops.nessai_amd.clip_grad_norm_(parameters, *args)

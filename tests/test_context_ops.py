@@ -165,3 +165,45 @@ def test_group_norm_refuses_more_workgroups_than_a_launch_holds():
     assert b"too many samples" in L.nsa_last_error()
     assert L.nsa_group_norm_backward(samples, 1, channels, channels, 1, ws, ws, 0, None, None, -1, ws, ws, ws, None, None, ws, 1 << 62, None) < 0
     assert b"too many samples" in L.nsa_last_error()
+
+
+def test_operators_of_tensors_without_data():
+    """Shapes, types and devices of results on the Meta key, and what a tracer records: the inner operators, whose schemas name
+    what they change."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def meta(*shape, dtype=torch.float32, **kw):
+        return torch.empty(*shape, dtype=dtype, device="meta", **kw)
+
+    with torch.enable_grad():
+        x, w, b = meta(4, 5, 12, dtype=torch.bfloat16, requires_grad=True), meta(12, requires_grad=True), meta(12, requires_grad=True)
+        y = ops.group_norm_act(x, 3, w, b, activation="silu")
+        assert y.shape == x.shape and y.dtype == torch.bfloat16 and y.is_meta and y.requires_grad
+        for wanted in ([x, w, b], [w], [x, b]):
+            grads = torch.autograd.grad(y, wanted, torch.empty_like(y), retain_graph=True)
+            assert [(g.shape, g.dtype) for g in grads] == [(v.shape, v.dtype) for v in wanted]
+        table, ids = meta(7, 3, dtype=torch.float16, requires_grad=True), meta(2, 3, dtype=torch.int32)
+        out = ops.embedding(ids, table, scale=2.0, padding_idx=-1)
+        assert out.shape == (2, 3, 3) and out.dtype == torch.float16
+        (g,) = torch.autograd.grad(out, [table], torch.empty_like(out))
+        assert g.shape == table.shape and g.dtype == table.dtype
+        p = torch.nn.Parameter(meta(4))
+        p.grad = meta(4)
+        for norm in (ops.grad_norm([p.grad, meta(3, dtype=torch.bfloat16)]), ops.clip_grad_norm_([p], 1.0)):
+            assert norm.shape == () and norm.dtype == torch.float32 and norm.is_meta
+        with pytest.raises(ValueError, match="cannot be divided"):
+            ops.group_norm_act(x, 5)
+
+        def step(ids, table, w, dy):
+            table, w = table.detach().requires_grad_(), w.detach().requires_grad_()
+            y = ops.group_norm_act(ops.embedding(ids, table), 4, w)
+            grads = torch.autograd.grad(y, [table, w], dy)
+            return y, torch.ops.nessai_amd.clip_grad_norm_of_([g.clone() for g in grads], 2, 1.0, False)
+
+        graph = make_fx(step)(meta(5, dtype=torch.int64), meta(7, 8), meta(8), meta(5, 8)).graph
+    called = [n.target._schema.name for n in graph.nodes if n.op == "call_function" and "nessai_amd" in str(n.target)]
+    assert called == [f"nessai_amd::_{k}" for k in ("embedding_forward", "group_norm_forward", "group_norm_backward",
+                                                    "embedding_backward", "clip_gradients_")]
+    for name in ("clip_grad_norm_of_", "_clip_gradients_"):
+        schema = getattr(torch.ops.nessai_amd, name).default._schema
+        assert schema.is_mutable and schema.arguments[0].alias_info.is_write

@@ -725,3 +725,32 @@ def test_group_norm_launches_in_two_dimensions():
     # (two terms; a chain of 257 values in a thread's sums, about a member of at most 6 spreads)
     assert bool(((db.double() - d.sum(0)).abs() <= 2 * U32 * d.abs().sum(0)).all())
     assert bool(((dw.double() - (d * xh).sum(0)).abs() <= 260 * U32 * (1 + 6) * (d.abs() * (1 + xh.abs())).sum(0)).all())
+
+
+# ---- traced ------------------------------------------------------------------------------------------------------------
+
+
+def test_a_compiled_pass_gives_the_eager_bits():
+    """torch.compile without a code generator: the traced graphs of the forward and the backward pass, run as they are."""
+    def forward(ids, table, w, b):
+        return ops.group_norm_act(ops.embedding(ids, table, scale=2.0), 4, w, b, activation="silu")
+
+    ids, table, w, b, dy = _chain_inputs(5)
+    want = [y := forward(ids, table, w, b), *torch.autograd.grad(y, [table, w, b], dy)]
+    compiled = torch.compile(forward, backend="aot_eager", fullgraph=True)
+    got = [y := compiled(ids, table, w, b), *torch.autograd.grad(y, [table, w, b], dy)]
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
+    with torch.no_grad():
+        assert torch.equal(compiled(ids, table, w, b), want[0])
+
+
+def test_a_compiled_clip_changes_the_gradients():
+    def clip(grads):
+        return torch.ops.nessai_amd.clip_grad_norm_of_(grads, 2, 0.5, False)
+
+    for dtypes in ([torch.float32], TYPES):
+        params, _ = _params(GRADS["minibatch_flow"], dtypes, "own")
+        ours = [p.grad.clone() for p in params]
+        want = ops.clip_grad_norm_(params, 0.5)
+        got = torch.compile(clip, backend="aot_eager", fullgraph=True)(ours)
+        assert torch.equal(want, got) and all(torch.equal(p.grad, g) for p, g in zip(params, ours))
