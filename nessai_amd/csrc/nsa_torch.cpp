@@ -356,7 +356,8 @@ Tensor norm_call(at::TensorList tensors, int64_t kind, bool clip, double max_nor
   long long elements = 0;
   for (int i = 0; i < count; ++i) {
     const Tensor& t = tensors[i];
-    places[i] = const_cast<void*>(t.const_data_ptr());
+    // (what is written is asked for as such: a lazy clone then gets memory of its own; the norm only reads)
+    places[i] = clip ? t.mutable_data_ptr() : const_cast<void*>(t.const_data_ptr());
     sizes[i] = t.numel();
     elements += sizes[i];
     codes[i] = dtype_code(t, "gradients");

@@ -161,6 +161,20 @@ def test_clip_of_gradients_in_other_orders_of_memory():
         ops.clip_grad_norm_([q], 1.0)
 
 
+def test_clip_of_a_lazy_clone_leaves_its_source():
+    for shape in ((100,), (300_001,)):
+        source = randn(*shape)
+        kept = source.clone()
+        p, q = torch.nn.Parameter(torch.zeros(shape, device=DEV)), torch.nn.Parameter(torch.zeros(shape, device=DEV))
+        p.grad, q.grad = torch._lazy_clone(source), torch._lazy_clone(source)
+        ref = math.sqrt(2) * float(kept.double().norm())
+        assert abs(float(ops.clip_grad_norm_([p, q], 0.5)) - ref) <= 4 * U32 * ref
+        assert torch.equal(source, kept)
+        for g in (p.grad, q.grad):  # (three operations of the factor, one product)
+            want = kept.double() * (0.5 / (ref + 1e-6))
+            assert bool(((g.double() - want).abs() <= 8 * U32 * want.abs()).all())
+
+
 def test_clip_is_seen_by_autograd():
     """A graph that saved a gradient notices that the clip changed it."""
     p = torch.nn.Parameter(torch.ones(3, device=DEV))
