@@ -15,6 +15,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <array>
 #include <cmath>
 #include <optional>
@@ -403,12 +404,21 @@ Tensor clip_(std::vector<Tensor> grads, int64_t kind, double max_norm, bool erro
   check_gradients(grads, "clip_grad_norm_: gradients");
   // a gradient with gaps between its elements is clipped in a copy; one whose elements share memory cannot be
   std::vector<Tensor> dense = grads;
+  bool copies = false;
   for (Tensor& g : dense) {
     if (g.is_non_overlapping_and_dense()) continue;
+    copies = true;
     for (int64_t d = 0; d < g.dim(); ++d)
       TORCH_CHECK_VALUE(g.stride(d) != 0 || g.size(d) <= 1,
                         "clip_grad_norm_: a gradient's elements overlap in memory (an expanded tensor); clone it");
     g = g.contiguous();
+  }
+  if (copies) {  // (the entry point sees those, not what they are copies of: one gradient given twice would pass)
+    std::vector<std::pair<const void*, int64_t>> first;
+    for (const Tensor& g : grads)
+      if (g.numel() > 0) first.emplace_back(g.storage().unsafeGetStorageImpl(), g.storage_offset());
+    std::sort(first.begin(), first.end());
+    TORCH_CHECK(std::adjacent_find(first.begin(), first.end()) == first.end(), "clip_grad_norm_: two gradients overlap in memory");
   }
   if (error_if_nonfinite)
     TORCH_CHECK(std::isfinite(call_total_norm(dense, kind).item<float>()),

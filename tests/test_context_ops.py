@@ -207,3 +207,16 @@ def test_operators_of_tensors_without_data():
     for name in ("clip_grad_norm_of_", "_clip_gradients_"):
         schema = getattr(torch.ops.nessai_amd, name).default._schema
         assert schema.is_mutable and schema.arguments[0].alias_info.is_write
+
+
+def test_clip_refuses_a_gradient_with_gaps_given_twice():
+    """It is clipped in a copy, of which the entry point's own check knows nothing.  Two views that interleave are apart."""
+    wide = torch.empty(6, 40, device="meta")
+    p, q = (torch.nn.Parameter(torch.empty(6, 20, device="meta")) for _ in range(2))
+    p.grad, q.grad = wide[:, ::2], wide[:, 1::2]
+    assert ops.clip_grad_norm_([p, q], 1.0).shape == ()
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.clip_grad_norm_([p, p], 1.0)
+    q.grad = wide[:, :20]
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.clip_grad_norm_([q, p], 1.0)
