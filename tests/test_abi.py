@@ -2,7 +2,7 @@
 import ctypes
 import os
 import re
-
+import subprocess
 
 from nessai_amd import lib, pack
 
@@ -39,6 +39,19 @@ def test_version_and_instance_query():
     assert L.nsa_flow_supported(2, 1, 7) == 1 and L.nsa_flow_generic_bins(2, 7) == 1  # the generic spline instance
     assert L.nsa_flow_generic_bins(2, 8) == 0 and L.nsa_flow_supported(2, 1, 17) == 0
     assert L.nsa_flow_supported(9, 1, 8) == 0
+
+
+def test_the_c_library_builds_without_torch():
+    """``make`` where python3 has no torch: the C ABI library's commands, and none that names torch's headers."""
+
+    def run(*args):
+        command = ["make", "-n", "-B", "-C", os.path.join(ROOT, "nessai_amd", "csrc"), *args]
+        return subprocess.run(command, capture_output=True, text=True, check=True).stdout
+
+    without, usual = run("TORCH_DIR="), run()
+    assert "nsa_embedding.hip" in without and "-o ../libnessai_amd.so" in without
+    assert "nsa_torch.cpp" not in without and "is not built" in without
+    assert "nsa_torch.cpp" in usual and "-o ../libnessai_amd_torch.so" in usual
 
 
 def test_max_key_roundtrip_is_monotone():
