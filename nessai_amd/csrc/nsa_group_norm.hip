@@ -94,9 +94,18 @@ __device__ __forceinline__ float gn_param(const void* p, int f32, int c, float n
 
 // Which workgroup of a launch this is.  A launch holds fewer than 2^32 threads in a dimension - 2^24 workgroups of 256, which
 // many samples of many groups pass - so more than GN_GRID_X workgroups lie in rows of as many (gn_grid); those behind the
-// last one have nothing to do, each as a whole.
+// last one have nothing to do, each as a whole.  (Not by gridDim: reading it costs a load before anything else can begin.)
 #define GN_GRID_X (1 << 20)
-__device__ __forceinline__ long long gn_block() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }
+__device__ __forceinline__ long long gn_block() { return (long long)blockIdx.y * GN_GRID_X + blockIdx.x; }
+
+// i = q d + r, in 32 bits where i fits (a division of 64 bits is a hundred instructions)
+__device__ __forceinline__ long long gn_split(long long i, int d, int& r) {
+  long long q;
+  if ((unsigned long long)i >> 32 == 0) q = (uint32_t)i / (uint32_t)d;
+  else q = i / d;
+  r = (int)(i - q * d);
+  return q;
+}
 
 struct GnPlace {  // what this workgroup works on
   long long n, l0, l1;  // n >= samples: nothing
@@ -106,11 +115,7 @@ struct GnPlace {  // what this workgroup works on
 
 __device__ __forceinline__ GnPlace gn_place(const GnShape& s) {
   GnPlace p;
-  long long b = gn_block();
-  p.chunk = (int)(b % s.chunks);
-  b /= s.chunks;
-  p.slab = (int)(b % s.slabs);
-  p.n = b / s.slabs;
+  p.n = gn_split(gn_split(gn_block(), s.chunks, p.chunk), s.slabs, p.slab);
   p.l0 = p.chunk * s.chunk;
   p.l1 = p.l0 + s.chunk < s.length ? p.l0 + s.chunk : s.length;
   p.j = threadIdx.x % s.vecs;
@@ -233,7 +238,8 @@ __global__ void __launch_bounds__(GN_THREADS) gn_stats_join(GnShape s, const flo
                                                             float* __restrict__ mean_out, float* __restrict__ rstd_out) {
   const long long i = gn_block() * (GN_THREADS / 64) + (threadIdx.x >> 6);
   if (i >= s.samples * s.groups) return;
-  const long long n = i / s.groups, g = i % s.groups;
+  int g;
+  const long long n = gn_split(i, s.groups, g);
   const int lane = threadIdx.x & 63;
   double mean = 0.0, m2 = 0.0, count = 0.0;
   auto join = [&](double mean_b, double m2_b, double count_b) {
@@ -353,9 +359,10 @@ __global__ void __launch_bounds__(GN_THREADS) gn_sums(GnShape s, const T* __rest
 __global__ void __launch_bounds__(GN_JOIN_THREADS) gn_sums_columns(GnShape s, float2* __restrict__ part) {
   __shared__ float2 red[GN_JOIN_THREADS];
   const int slabs = (s.channels + 63) / 64, share = threadIdx.x >> 6;
-  const long long n = gn_block() / slabs;
+  int slab;
+  const long long n = gn_split(gn_block(), slabs, slab);
   if (n >= s.samples) return;
-  const int c = (int)(gn_block() % slabs) * 64 + (threadIdx.x & 63);
+  const int c = slab * 64 + (threadIdx.x & 63);
   float2* p = part + n * s.chunks * s.channels + c;
   float2 a = make_float2(0.0f, 0.0f);
   if (c < s.channels) {
@@ -383,9 +390,10 @@ __global__ void __launch_bounds__(GN_THREADS) gn_sums_join(GnShape s, int chunks
                                                            GnParams q,
                                                            float2* __restrict__ ab) {
   __shared__ float2 red[GN_THREADS];
-  const long long pair = gn_block(), n = pair / s.groups;
+  int g;
+  const long long pair = gn_block(), n = gn_split(pair, s.groups, g);
   if (n >= s.samples) return;
-  const int g = (int)(pair % s.groups), lane = threadIdx.x % across, share = threadIdx.x / across;
+  const int lane = threadIdx.x % across, share = threadIdx.x / across;
   const int shares = GN_THREADS / across;
   float2 t = make_float2(0.0f, 0.0f);  // this thread's part of A and B
   for (int base = 0; base < s.cpg; base += across) {
