@@ -6,7 +6,8 @@
 // Nothing here computes.  The public operators check their arguments and record for autograd; each calls one of the inner
 // ones (a leading underscore), which exist for the CUDA (ROCm) dispatch key - results and workspaces are allocated and one
 // entry point called on the current stream of the tensors' device - and for the Meta key, where they return the results'
-// shapes.  The public ones have one body for every key, so a tracer (torch.compile, make_fx) sees the inner ones.
+// shapes.  The public ones have one body for every key, so a tracer (torch.compile, make_fx) sees the inner ones; those check
+// by themselves what the kernels rely on, because a traced graph calls them with tensors of its own.
 // The entry points' addresses come from the loaded libnessai_amd.so (nessai_amd/lib.py).
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
@@ -91,6 +92,11 @@ struct Inner {
 
 std::optional<Tensor> given(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 
+// what a kernel relies on, in an inner operator
+void expect(bool holds, const char* what, const char* condition) {
+  TORCH_CHECK(holds, "nessai_amd::", what, ": expected ", condition);
+}
+
 const void* data(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* mutable_data(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 
@@ -125,6 +131,20 @@ int param_dtype(const Tensor& weight, const Tensor& bias) {
   return p.defined() ? dtype_code(p, "group_norm_act: weight") : NSA_DT_F32;
 }
 
+void expect_group_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias,
+                       int64_t groups, const char* what) {
+  expect(x.dim() >= 2 && x.is_contiguous(), what, "a contiguous x of two dimensions or more");
+  const int64_t channels = x.size(-1);
+  expect(groups >= 1 && channels >= 1 && channels <= (1 << 30) && channels % groups == 0, what, "channels in whole groups");
+  for (const auto* p : {&weight, &bias})
+    if (p->has_value())
+      expect((*p)->is_contiguous() && (*p)->dim() == 1 && (*p)->size(0) == channels && (*p)->device() == x.device() &&
+                 ((*p)->scalar_type() == at::kFloat || (*p)->scalar_type() == x.scalar_type()),
+             what, "a contiguous weight and bias of x's channels, on its device, in float32 or its type");
+  expect(!weight.has_value() || !bias.has_value() || weight->scalar_type() == bias->scalar_type(), what,
+         "a weight and a bias of one type");
+}
+
 std::tuple<Tensor, Tensor> group_norm_results(const Tensor& x, int64_t groups) {
   return {at::empty(x.sizes(), x.options()), at::empty({2, Rows(x).samples, groups}, x.options().dtype(at::kFloat))};
 }
@@ -133,6 +153,7 @@ std::tuple<Tensor, Tensor> group_norm_results(const Tensor& x, int64_t groups) {
 std::tuple<Tensor, Tensor> group_norm_forward(const Tensor& x, const std::optional<Tensor>& weight_,
                                               const std::optional<Tensor>& bias_, int64_t groups, double eps,
                                               int64_t activation) {
+  expect_group_norm(x, weight_, bias_, groups, "_group_norm_forward");
   const Rows r(x);
   const Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
   auto results = group_norm_results(x, groups);
@@ -150,14 +171,23 @@ std::tuple<Tensor, Tensor> group_norm_forward(const Tensor& x, const std::option
   return results;
 }
 
-std::tuple<Tensor, Tensor> group_norm_forward_meta(const Tensor& x, const std::optional<Tensor>&, const std::optional<Tensor>&,
-                                                   int64_t groups, double, int64_t) {
+std::tuple<Tensor, Tensor> group_norm_forward_meta(const Tensor& x, const std::optional<Tensor>& weight,
+                                                   const std::optional<Tensor>& bias, int64_t groups, double, int64_t) {
+  expect_group_norm(x, weight, bias, groups, "_group_norm_forward");
   return group_norm_results(x, groups);
 }
 
 // dx, dweight, dbias: undefined where they are not wanted
-std::tuple<Tensor, Tensor, Tensor> group_norm_gradients(const Tensor& x, const std::optional<Tensor>& weight,
-                                                        const std::optional<Tensor>& bias, std::array<bool, 3> wanted) {
+std::tuple<Tensor, Tensor, Tensor> group_norm_gradients(const Tensor& dy, const Tensor& x, const std::optional<Tensor>& weight,
+                                                        const std::optional<Tensor>& bias, const Tensor& stats, int64_t groups,
+                                                        int64_t, std::array<bool, 3> wanted) {
+  const char* what = "_group_norm_backward";
+  expect_group_norm(x, weight, bias, groups, what);
+  expect(dy.is_contiguous() && dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type() && dy.device() == x.device(),
+         what, "a contiguous dy of x's shape, type and device");
+  expect(stats.is_contiguous() && stats.numel() == 2 * x.size(0) * groups && stats.scalar_type() == at::kFloat &&
+             stats.device() == x.device(),
+         what, "the forward pass's statistics");
   auto like = [](bool want, const std::optional<Tensor>& t) {
     return want && t.has_value() ? at::empty(t->sizes(), t->options()) : Tensor();
   };
@@ -167,10 +197,10 @@ std::tuple<Tensor, Tensor, Tensor> group_norm_gradients(const Tensor& x, const s
 std::tuple<Tensor, Tensor, Tensor> group_norm_backward(const Tensor& dy, const Tensor& x, const std::optional<Tensor>& weight_,
                                                        const std::optional<Tensor>& bias_, const Tensor& stats,
                                                        int64_t groups, int64_t activation, std::array<bool, 3> wanted) {
+  auto results = group_norm_gradients(dy, x, weight_, bias_, stats, groups, activation, wanted);
   const Rows r(x);
   const Tensor weight = weight_.value_or(Tensor()), bias = bias_.value_or(Tensor());
   const c10::DeviceGuard guard(x.device());
-  auto results = group_norm_gradients(x, weight_, bias_, wanted);
   const auto& [dx, dw, db] = results;
   const int code = dtype_code(x, "group_norm_act: x");
   const size_t size = g_entry.group_norm_workspace(r.samples, r.length, r.channels, groups, code, 1);
@@ -182,12 +212,6 @@ std::tuple<Tensor, Tensor, Tensor> group_norm_backward(const Tensor& dy, const T
                                     ws.mutable_data_ptr(), size, stream_of(x)),
         "nsa_group_norm_backward");
   return results;
-}
-
-std::tuple<Tensor, Tensor, Tensor> group_norm_backward_meta(const Tensor&, const Tensor& x, const std::optional<Tensor>& weight,
-                                                            const std::optional<Tensor>& bias, const Tensor&, int64_t, int64_t,
-                                                            std::array<bool, 3> wanted) {
-  return group_norm_gradients(x, weight, bias, wanted);
 }
 
 std::tuple<Tensor, Tensor> call_group_norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups,
@@ -256,6 +280,10 @@ Tensor group_norm_act(const Tensor& x_, int64_t groups, const std::optional<Tens
 // -- embedding --------------------------------------------------------------------------------------------------------
 
 Tensor embedding_rows(const Tensor& ids, const Tensor& weight, double) {
+  expect(ids.is_contiguous() && (ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong), "_embedding_forward",
+         "contiguous int32 or int64 indices");
+  expect(weight.is_contiguous() && weight.dim() == 2 && weight.device() == ids.device(), "_embedding_forward",
+         "a contiguous table on the indices' device");
   std::vector<int64_t> shape = ids.sizes().vec();
   shape.push_back(weight.size(1));
   return at::empty(shape, weight.options());
@@ -272,7 +300,12 @@ Tensor embedding_forward(const Tensor& ids, const Tensor& weight, double scale) 
   return out;
 }
 
-Tensor embedding_table(const Tensor& dy, const Tensor&, int64_t vocab, int64_t width, double, int64_t) {
+Tensor embedding_table(const Tensor& dy, const Tensor& ids, int64_t vocab, int64_t width, double, int64_t) {
+  expect(ids.is_contiguous() && (ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong), "_embedding_backward",
+         "contiguous int32 or int64 indices");
+  expect(vocab >= 1 && width >= 1 && width <= (1 << 20) && dy.is_contiguous() && dy.numel() == ids.numel() * width &&
+             dy.device() == ids.device(),
+         "_embedding_backward", "a contiguous dy of a row for each index, on their device");
   return at::empty({vocab, width}, dy.options());
 }
 
@@ -347,8 +380,14 @@ void check_gradients(const std::vector<Tensor>& tensors, const char* what) {
   on_device(tensors[0], what);
 }
 
+void expect_dense(at::TensorList tensors, const char* what) {
+  for (const Tensor& t : tensors)
+    expect(t.is_non_overlapping_and_dense() && t.device() == tensors[0].device(), what, "dense tensors on one device");
+}
+
 // clip: by max_norm, in place; otherwise the norm alone.  Every tensor fills one stretch of memory.
 Tensor norm_call(at::TensorList tensors, int64_t kind, bool clip, double max_norm) {
+  expect_dense(tensors, clip ? "_clip_gradients_" : "_total_norm");
   const c10::DeviceGuard guard(tensors[0].device());
   const int count = (int)tensors.size();
   std::vector<void*> places(count);
@@ -379,7 +418,10 @@ Tensor norm_call(at::TensorList tensors, int64_t kind, bool clip, double max_nor
 
 Tensor total_norm(at::TensorList tensors, int64_t kind) { return norm_call(tensors, kind, false, 0.0); }
 Tensor clip_gradients(at::TensorList tensors, int64_t kind, double max_norm) { return norm_call(tensors, kind, true, max_norm); }
-Tensor total_norm_meta(at::TensorList tensors, int64_t) { return at::empty({}, tensors[0].options().dtype(at::kFloat)); }
+Tensor total_norm_meta(at::TensorList tensors, int64_t) {
+  expect_dense(tensors, "_total_norm");
+  return at::empty({}, tensors[0].options().dtype(at::kFloat));
+}
 Tensor clip_gradients_meta(at::TensorList tensors, int64_t kind, double) { return total_norm_meta(tensors, kind); }
 
 Tensor call_total_norm(at::TensorList tensors, int64_t kind) {
@@ -479,7 +521,7 @@ TORCH_LIBRARY_IMPL(nessai_amd, CUDA, m) {
 
 TORCH_LIBRARY_IMPL(nessai_amd, Meta, m) {
   m.impl("_group_norm_forward", &group_norm_forward_meta);
-  m.impl("_group_norm_backward", &group_norm_backward_meta);
+  m.impl("_group_norm_backward", &group_norm_gradients);
   m.impl("_embedding_forward", &embedding_rows);
   m.impl("_embedding_backward", &embedding_table);
   m.impl("_total_norm", &total_norm_meta);

@@ -220,3 +220,42 @@ def test_clip_refuses_a_gradient_with_gaps_given_twice():
     q.grad = wide[:, :20]
     with pytest.raises(RuntimeError, match="overlap"):
         ops.clip_grad_norm_([q, p], 1.0)
+
+
+def test_inner_operators_check_what_their_kernels_rely_on():
+    """A traced graph calls them with tensors of its own: strides, shapes, types and devices are checked there as well."""
+    def meta(*shape, dtype=torch.float32):
+        return torch.empty(*shape, dtype=dtype, device="meta")
+
+    o = torch.ops.nessai_amd
+    x, w, stats = meta(4, 5, 12), meta(12), meta(2, 4, 3)
+    wanted = [True, True, True]
+    assert o._group_norm_forward(x, w, w, 3, 1e-5, 0)[1].shape == (2, 4, 3)
+    assert [g.shape for g in o._group_norm_backward(x, x, w, w, stats, 3, 0, wanted)] == [(4, 5, 12), (12,), (12,)]
+    ids, dy = meta(6, dtype=torch.int64), meta(6, 3)
+    assert o._embedding_forward(ids, meta(7, 3), 1.0).shape == (6, 3) and o._embedding_backward(dy, ids, 7, 3, 1.0, -1).shape == (7, 3)
+    wide = meta(4, 5, 24)[..., ::2]
+    for call in (
+        lambda: o._group_norm_forward(wide, w, w, 3, 1e-5, 0),
+        lambda: o._group_norm_forward(x, meta(24)[::2], None, 3, 1e-5, 0),
+        lambda: o._group_norm_forward(x, meta(11), None, 3, 1e-5, 0),
+        lambda: o._group_norm_forward(x, w, meta(12, dtype=torch.bfloat16), 3, 1e-5, 0),
+        lambda: o._group_norm_forward(x, w, torch.empty(12), 3, 1e-5, 0),
+        lambda: o._group_norm_forward(x, w, w, 5, 1e-5, 0),
+        lambda: o._group_norm_backward(wide, x, w, w, stats, 3, 0, wanted),
+        lambda: o._group_norm_backward(meta(4, 5, 11), x, w, w, stats, 3, 0, wanted),
+        lambda: o._group_norm_backward(x.bfloat16(), x, w, w, stats, 3, 0, wanted),
+        lambda: o._group_norm_backward(x, x, w, w, meta(4, 3), 3, 0, wanted),
+        lambda: o._embedding_forward(ids.int()[::2], meta(7, 3), 1.0),
+        lambda: o._embedding_forward(dy, meta(7, 3), 1.0),
+        lambda: o._embedding_forward(ids, meta(3, 7).t(), 1.0),
+        lambda: o._embedding_backward(meta(3, 6).t(), ids, 7, 3, 1.0, -1),
+        lambda: o._embedding_backward(meta(5, 3), ids, 7, 3, 1.0, -1),
+        lambda: o._embedding_backward(dy, ids, 0, 3, 1.0, -1),
+        lambda: o._total_norm([w, meta(24)[::2]], 2),
+        lambda: o._clip_gradients_([w, meta(24)[::2]], 2, 1.0),
+    ):
+        with pytest.raises(RuntimeError, match="expected"):
+            call()
+    with pytest.raises(RuntimeError, match="empty list"):  # (the dispatcher's own refusal)
+        o._total_norm([], 2)

@@ -758,6 +758,15 @@ def test_a_compiled_pass_gives_the_eager_bits():
         assert torch.equal(compiled(ids, table, w, b), want[0])
 
 
+def test_a_compiled_clip_of_parameters():
+    """The gradients of parameters that a compiled function is given."""
+    params, _ = _params(GRADS["minibatch_flow"], [torch.float32], "own")
+    others, _ = _params(GRADS["minibatch_flow"], [torch.float32], "own")
+    want = ops.clip_grad_norm_(params, 0.5)
+    got = torch.compile(lambda ps: ops.clip_grad_norm_(ps, 0.5), backend="aot_eager")(others)
+    assert torch.equal(want, got) and all(torch.equal(p.grad, q.grad) for p, q in zip(params, others))
+
+
 def test_a_compiled_clip_changes_the_gradients():
     def clip(grads):
         return torch.ops.nessai_amd.clip_grad_norm_of_(grads, 2, 0.5, False)
