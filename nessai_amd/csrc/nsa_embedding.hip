@@ -10,8 +10,9 @@
 // table's size has digits - and the sums then run over neighbours, in the order of the positions: equal inputs give equal
 // bits.  The sorted list is cut into chunks of equal length, whatever the frequencies of the ids: an id inside one chunk
 // is finished there; one that runs over a chunk's border leaves float32 partial sums, which a second kernel joins.
-// 131072 rows of 320 bfloat16 into 32768 (84 MB in, 21 MB out): 61 us; sorting and clearing 2 x 12, adding 21, joining 13.  The
-// sort is bound by the latency of its short kernels, the sums by gathering rows (4.0 TB/s).
+// 131072 rows of 320 bfloat16 into 32768 (84 MB in, 21 MB out): 61 us; sorting and clearing 15 + 12, adding 21, joining 13.
+// The sums are bound by gathering rows (4.0 TB/s), the sort of so few tokens by the latency of its short kernels.  Sorting
+// 10^6 tokens into 5000 takes 43 us (counts 14, scans 10, scatters 19) for 48 MB read and written.
 #include <hip/hip_runtime.h>
 #include <algorithm>
 

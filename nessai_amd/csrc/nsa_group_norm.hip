@@ -38,7 +38,7 @@ __device__ __forceinline__ float gn_sigmoid(float z) {
 }
 
 // 2 / (1 + e^-2z) - 1; near zero, where that is a difference of equal numbers, the series z - z^3/3 + 2 z^5/15 - 17 z^7/315
-// (the next term is 62 z^9 / 2835: below 2^-28 of z at the border)
+// (the next term is 62 z^9 / 2835: below 2^-27 of z at the border)
 __device__ __forceinline__ float gn_tanh(float z) {
   const float s = z * z;
   const float near = z * fmaf(s, fmaf(s, fmaf(s, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
