@@ -227,6 +227,7 @@ def test_inner_operators_check_what_their_kernels_rely_on():
     def meta(*shape, dtype=torch.float32):
         return torch.empty(*shape, dtype=dtype, device="meta")
 
+    lib.load_torch()
     o = torch.ops.nessai_amd
     x, w, stats = meta(4, 5, 12), meta(12), meta(2, 4, 3)
     wanted = [True, True, True]
